@@ -6,6 +6,7 @@ call fails, an exception is raised; nothing falls back to the CPU.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -16,6 +17,8 @@ GGML_F32, GGML_Q4_0, GGML_Q8_0, GGML_Q4_K, GGML_Q6_K = 0, 2, 8, 12, 14
 GGML_TO_MAT = {GGML_F32: MAT_F32, GGML_Q4_0: MAT_Q4, GGML_Q8_0: MAT_Q8, GGML_Q4_K: MAT_Q4K, GGML_Q6_K: MAT_Q6K}
 
 _vp, _u32, _sz, _int, _f32 = C.c_void_p, C.c_uint32, C.c_size_t, C.c_int, C.c_float
+# ie_b200_kv_pages: kp, vp, table, (n_pages, page, n_kv, hd, n_seq, table_cols, table_stride), kv_f32, page_stride
+KV_PAGES = struct.Struct("@PPP7IiN")
 
 # name -> (restype, argtypes); every symbol include/ie_b200.h declares
 SIGNATURES = {
@@ -53,6 +56,9 @@ SIGNATURES = {
     "ie_b200_attn_prefill": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _sz, _sz, _sz, _vp]),
     "ie_b200_attn_prefill_scratch_bytes": (_sz, [_u32, _u32, _u32]),
     "ie_b200_attn_prefill_split": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _sz, _sz, _sz, _u32, _vp, _vp, _vp]),
+    "ie_b200_rope_kv_paged": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _u32, _vp, _vp, _u32, _int, _u32, _sz, _sz, _vp, _vp]),
+    "ie_b200_attn_decode_paged_scratch_bytes": (_sz, [_u32, _u32, _u32]),
+    "ie_b200_attn_decode_paged": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _sz, _sz, _sz, _vp, _vp, _vp]),
     "ie_b200_argmax_part_bytes": (_sz, [_u32]),
     "ie_b200_argmax": (_int, [_vp, _u32, _vp, _u32, _sz, _sz, _vp, _vp]),
     "ie_b200_topk_scratch_bytes": (_sz, [_u32, _u32, _u32]),

@@ -1,0 +1,557 @@
+// attn_paged.cu -- attention of one new token per row over a paged KV cache, for a batch of rows of any lengths.
+//
+// For row r and query head h of KV head g: out = sum_p w_p v_p / sum_p w_p with w_p = exp(q . k_p / sqrt(hd) - max), over the
+// positions p < len[r] of its sequence. K and V of a KV head are read once for all its query heads (up to eight; more come in groups,
+// the later of which find the rows in L2). Bound: HBM, 2 len n_kv hd sizeof(KV) bytes a row.
+//
+// Work. A chunk is CH positions of one (row, KV head, head group); pages hold whole chunks, so a chunk is one contiguous run of K and
+// one of V. All chunks of the batch, in that order, are cut into even shares, one per CTA, wherever the cuts fall: the CTAs finish
+// together whatever the lengths are. A CTA finds its share by a prefix sum over the rows' lengths. Its four warps take the chunks of
+// a unit (row, KV head, group) in turn; each warp has its own ring of buffers that it fills itself (cp.async, rows past the length
+// zero-filled) and its own running maximum, sum and outputs, so nothing in the stream waits for another warp, and the ring runs on into
+// the next unit while this one's records are merged. A unit that lies in one CTA is finished there; the parts of a cut one go to
+// global memory as (outputs, max, sum) records, and the CTA that finishes last adds them in the order of the positions.
+//
+// Half cache: mma.sync m16n8k16, the positions on the 16-row side, the heads on the 8-column side (as attn_decode.cu). q and the
+// weights are carried as two f16 terms; every accumulation takes few MMAs (what the tensor cores cut off grows with their number) and is
+// added up in fp32: S in three chains (low terms, even and odd steps of the high ones), O per chunk. Weights are scaled by 2^15
+// before they are split, so that the low term of a small one keeps its bits (f16's subnormals end at 2^-24).
+// Float cache: the same with fp32 FMAs, four lanes per position.
+#include <cuda_pipeline_primitives.h>
+#include <math.h>
+
+#include "paged.cuh"
+#include "row_store.cuh"
+
+namespace ieb {
+
+constexpr int AP_WARPS = 4, AP_THREADS = 32 * AP_WARPS, AP_STAGES = 3, AP_HEADS = 8;
+constexpr uint32_t AP_MAX_CTAS = 1024u;  // the counters at the front of the scratch
+
+struct PagedAttnArgs {
+  const float *q;
+  float *out, *rec;
+  uint8_t *oq;
+  const uint32_t *len, *seq;
+  uint32_t *count, *err;
+  ie_b200_kv_pages kv;
+  uint32_t n_head, G, groups, gw, R, wide;  // groups: head groups of a KV head, gw heads each (the last may have fewer)
+  uint32_t min_share;
+  size_t q_stride, out_stride, oq_stride;
+  float scale_log2;  // log2(e) / sqrt(hd)
+};
+
+template <typename KV, int HD>
+struct ApGeom {
+  static constexpr bool F16 = sizeof(KV) == 2;
+  static constexpr int CH = F16 ? 16 : 8;                       // positions of a chunk
+  static constexpr int ROWB = HD * (int)sizeof(KV), PIECES = ROWB / 16, PER_LANE = CH * PIECES / 32;
+  static constexpr int STAGE = 2 * CH * ROWB;                   // K rows, then V rows
+  static constexpr int RED_ROW = HD + 4;                        // floats between the heads of a record (banks: 4 per head pair)
+  static constexpr int RING_OFF = 0, RED_OFF = AP_WARPS * AP_STAGES * STAGE, ML_OFF = RED_OFF + AP_WARPS * AP_HEADS * RED_ROW * 4,
+                       VALID_OFF = ML_OFF + AP_WARPS * AP_HEADS * 8, MISC_OFF = VALID_OFF + AP_WARPS * AP_STAGES * 4, TOTAL = MISC_OFF + 64,
+                       Q_OFF = RED_OFF;  // float cache: the unit's q, until its records are written
+  static constexpr int FIT = 228 * 1024 / (TOTAL + 1024), CTAS = FIT < 4 ? FIT : 4;  // CTAs that an SM's shared memory holds
+  // The 16-byte pieces of a row change places so that the reads of eight rows (ldmatrix), or of two rows by four lanes each, meet
+  // eight different bank groups.
+  __device__ static __forceinline__ uint32_t at(uint32_t row, uint32_t piece) {
+    const uint32_t x = F16 ? (HD == 32 ? (row >> 1) & 3u : row & 7u) : (row & 1u) * 4u;
+    return row * ROWB + ((piece ^ x) * 16u);
+  }
+};
+
+__device__ __forceinline__ void ap_ldsm4(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ap_ldsm4t(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ uint32_t ap_movm_t(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ void ap_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ap_split2(float x, float y, uint32_t &hi, uint32_t &lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 hf = __half22float2(h);
+  const __half2 l = __floats2half2_rn(x - hf.x, y - hf.y);
+  hi = *reinterpret_cast<const uint32_t *>(&h), lo = *reinterpret_cast<const uint32_t *>(&l);
+}
+
+// ---- a warp's part of the arithmetic: its running maximum (log2 units), sum and outputs of the unit's heads
+template <typename KV, int HD>
+struct ApWarp;
+
+template <int HD>
+struct ApWarp<__half, HD> {
+  using Gm = ApGeom<__half, HD>;
+  static constexpr int KS = HD / 16;
+  uint32_t qh[KS][2], ql[KS][2];  // B fragments of Q^T[16 dims x heads]: column lane / 4
+  float o[KS][4], m[2], l[2];     // o[u][j], o[u][2 + j]: head 2 (lane % 4) + j, dims 16 u + lane / 4, + 8
+
+  __device__ __forceinline__ void start(const float *q, uint32_t heads, const uint8_t *, int lane) {
+    const uint32_t h = lane >> 2, tq = lane & 3;
+#pragma unroll
+    for (int k = 0; k < KS; k++) {
+      float2 a = make_float2(0.f, 0.f), b = a;
+      if (h < heads) {
+        a = *reinterpret_cast<const float2 *>(q + h * HD + 16 * k + 2 * tq);
+        b = *reinterpret_cast<const float2 *>(q + h * HD + 16 * k + 2 * tq + 8);
+      }
+      ap_split2(a.x, a.y, qh[k][0], ql[k][0]);
+      ap_split2(b.x, b.y, qh[k][1], ql[k][1]);
+#pragma unroll
+      for (int e = 0; e < 4; e++) o[k][e] = 0.0f;
+    }
+    m[0] = m[1] = -INFINITY, l[0] = l[1] = 0.0f;
+  }
+  __device__ __forceinline__ void chunk(const uint8_t *stage, uint32_t valid, float scale_log2, int lane) {
+    const uint32_t kb = smem_u32(stage), vb = kb + Gm::CH * Gm::ROWB, lm = lane >> 3, lr = lane & 7, hq = lane >> 2;
+    float sl[4] = {0.f, 0.f, 0.f, 0.f}, s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < KS; k++) {
+      uint32_t a[4];  // (positions lo, dims lo), (positions hi, dims lo), (positions lo, dims hi), (positions hi, dims hi)
+      ap_ldsm4(a, kb + Gm::at((lm & 1) * 8 + lr, 2 * k + (lm >> 1)));
+      ap_mma(sl, a, ql[k][0], ql[k][1]);
+      if (k & 1) ap_mma(s1, a, qh[k][0], qh[k][1]);
+      else ap_mma(s0, a, qh[k][0], qh[k][1]);
+    }
+    float s[4], p[4], al[2];  // s[j]: position lane / 4, s[2 + j]: + 8, of head 2 (lane % 4) + j
+#pragma unroll
+    for (int e = 0; e < 4; e++) s[e] = (s0[e] + s1[e]) + sl[e];
+    if (valid < 16u) {
+      if (hq >= valid) s[0] = s[1] = -INFINITY;
+      if (hq + 8u >= valid) s[2] = s[3] = -INFINITY;
+    }
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      float mx = fmaxf(s[j], s[2 + j]);
+      mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 4));
+      mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 8));
+      mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 16));
+      const float m_new = fmaxf(m[j], mx * scale_log2), base = m_new == -INFINITY ? 0.0f : m_new;
+      al[j] = ex2(m[j] - base);
+      p[j] = ex2(fmaf(s[j], scale_log2, -base)), p[2 + j] = ex2(fmaf(s[2 + j], scale_log2, -base));
+      l[j] = fmaf(l[j], al[j], p[j] + p[2 + j]);  // (of this lane's positions: the lanes meet in finish())
+      m[j] = m_new;
+    }
+    uint32_t ph[2], pl[2];  // each 8 x 8 block [positions x heads] transposed into the B fragment [positions x heads]
+    ap_split2(p[0] * 0x1p15f, p[1] * 0x1p15f, ph[0], pl[0]);
+    ap_split2(p[2] * 0x1p15f, p[3] * 0x1p15f, ph[1], pl[1]);
+#pragma unroll
+    for (int e = 0; e < 2; e++) ph[e] = ap_movm_t(ph[e]), pl[e] = ap_movm_t(pl[e]);
+#pragma unroll
+    for (int u = 0; u < KS; u++) {
+      uint32_t a[4];  // transposed on load: (dims lo, positions lo), (dims hi, positions lo), (dims lo, positions hi), (dims hi, positions hi)
+      ap_ldsm4t(a, vb + Gm::at((lm >> 1) * 8 + lr, 2 * u + (lm & 1)));
+      float c[4] = {0.f, 0.f, 0.f, 0.f};
+      ap_mma(c, a, pl[0], pl[1]);
+      ap_mma(c, a, ph[0], ph[1]);
+#pragma unroll
+      for (int e = 0; e < 4; e++) o[u][e] = fmaf(o[u][e], al[e & 1], c[e]);
+    }
+  }
+  // this warp's record: red [heads][RED_ROW] outputs (2^15 times), ml [heads][2]
+  __device__ __forceinline__ void finish(float *red, float *ml, int lane) {
+    const uint32_t hq = lane >> 2, tq = lane & 3;
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      float sum = l[j];
+      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 4);
+      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 8);
+      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 16);
+      const uint32_t h = 2 * tq + j;
+#pragma unroll
+      for (int u = 0; u < KS; u++) red[h * Gm::RED_ROW + 16 * u + hq] = o[u][j], red[h * Gm::RED_ROW + 16 * u + hq + 8] = o[u][2 + j];
+      if (hq == 0) ml[2 * h] = m[j], ml[2 * h + 1] = sum * 0x1p15f;
+    }
+  }
+};
+
+template <int HD>
+struct ApWarp<float, HD> {
+  using Gm = ApGeom<float, HD>;
+  static constexpr int DPL = HD / 32;  // output dims of a lane
+  float o[AP_HEADS][DPL], m[AP_HEADS], l[AP_HEADS];
+  const float *qs;
+
+  __device__ __forceinline__ void start(const float *, uint32_t, const uint8_t *q_smem, int) {
+    qs = reinterpret_cast<const float *>(q_smem);
+#pragma unroll
+    for (int h = 0; h < AP_HEADS; h++) {
+      m[h] = -INFINITY, l[h] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < DPL; d++) o[h][d] = 0.0f;
+    }
+  }
+  __device__ __forceinline__ void chunk(uint8_t *stage, uint32_t valid, float scale_log2, int lane) {
+    const uint32_t pos = lane >> 2, part = lane & 3;  // lane: a quarter of the dims of one position
+    float s[AP_HEADS], al[AP_HEADS];
+#pragma unroll
+    for (int h = 0; h < AP_HEADS; h++) s[h] = 0.0f;
+#pragma unroll 4
+    for (int i = 0; i < HD / 16; i++) {
+      const uint32_t piece = 4 * i + part;
+      const float4 k = *reinterpret_cast<const float4 *>(stage + Gm::at(pos, piece));
+#pragma unroll
+      for (int h = 0; h < AP_HEADS; h++) {
+        const float4 x = *reinterpret_cast<const float4 *>(qs + h * HD + 4 * piece);
+        s[h] = fmaf(x.x, k.x, s[h]), s[h] = fmaf(x.y, k.y, s[h]), s[h] = fmaf(x.z, k.z, s[h]), s[h] = fmaf(x.w, k.w, s[h]);
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < AP_HEADS; h++) {
+      s[h] += __shfl_xor_sync(0xFFFFFFFFu, s[h], 1);
+      s[h] += __shfl_xor_sync(0xFFFFFFFFu, s[h], 2);
+      if (pos >= valid) s[h] = -INFINITY;
+      float mx = s[h];
+      mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 4));
+      mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 8));
+      mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 16));
+      const float m_new = fmaxf(m[h], mx * scale_log2), base = m_new == -INFINITY ? 0.0f : m_new;
+      al[h] = ex2(m[h] - base);
+      s[h] = ex2(fmaf(s[h], scale_log2, -base));  // from here on the weight
+      l[h] = fmaf(l[h], al[h], s[h]);             // (of this lane's position: the lanes meet in finish())
+      m[h] = m_new;
+    }
+    // The weights [position][head] where the K rows were: every lane has read its part of them.
+    __syncwarp();
+    if (part == 0) {
+#pragma unroll
+      for (int h = 0; h < AP_HEADS; h += 4) *reinterpret_cast<float4 *>(stage + pos * 32u + 4 * h) = make_float4(s[h], s[h + 1], s[h + 2], s[h + 3]);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int h = 0; h < AP_HEADS; h++)
+#pragma unroll
+      for (int d = 0; d < DPL; d++) o[h][d] *= al[h];
+    const uint8_t *vs = stage + Gm::CH * Gm::ROWB;
+#pragma unroll
+    for (int j = 0; j < Gm::CH; j++) {
+      float v[DPL], w[AP_HEADS];
+      const uint8_t *at = vs + Gm::at(j, (lane * DPL) / 4) + ((lane * DPL) & 3) * 4;
+      if (DPL == 4) {
+        const float4 x = *reinterpret_cast<const float4 *>(at);
+        v[0] = x.x, v[1 % DPL] = x.y, v[2 % DPL] = x.z, v[3 % DPL] = x.w;
+      } else if (DPL == 2) {
+        const float2 x = *reinterpret_cast<const float2 *>(at);
+        v[0] = x.x, v[1 % DPL] = x.y;
+      } else {
+        v[0] = *reinterpret_cast<const float *>(at);
+      }
+#pragma unroll
+      for (int h = 0; h < AP_HEADS; h += 4) {
+        const float4 x = *reinterpret_cast<const float4 *>(stage + j * 32u + 4 * h);
+        w[h] = x.x, w[h + 1] = x.y, w[h + 2] = x.z, w[h + 3] = x.w;
+      }
+#pragma unroll
+      for (int h = 0; h < AP_HEADS; h++)
+#pragma unroll
+        for (int d = 0; d < DPL; d++) o[h][d] = fmaf(w[h], v[d], o[h][d]);
+    }
+  }
+  __device__ __forceinline__ void finish(float *red, float *ml, int lane) {
+#pragma unroll
+    for (int h = 0; h < AP_HEADS; h++) {
+      float sum = l[h];
+      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 4);
+      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 8);
+      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 16);
+#pragma unroll
+      for (int d = 0; d < DPL; d++) red[h * Gm::RED_ROW + lane * DPL + d] = o[h][d];
+      if (lane == 0) ml[2 * h] = m[h], ml[2 * h + 1] = sum;
+    }
+  }
+};
+
+// Where a CTA's share stands: chunks [j, j1) of unit `unit` of row r (this share's part of it), and what is left behind them.
+struct ApCursor {
+  uint32_t r, seq, len, unit, j0, j1;
+  uint64_t left;
+};
+
+// Positions and sequence of row r: 0 positions where the row pads the batch.
+__device__ __forceinline__ uint32_t ap_row(const PagedAttnArgs &a, uint32_t r, uint32_t &seq) {
+  seq = a.seq ? __ldg(a.seq + r) : r;
+  return seq < a.kv.n_seq ? min(__ldg(a.len + r), table_positions(a.kv)) : 0u;
+}
+
+template <typename KV, int HD>
+__global__ void __launch_bounds__(AP_THREADS, ApGeom<KV, HD>::CTAS) attn_paged_kernel(const PagedAttnArgs a) {
+  using Gm = ApGeom<KV, HD>;
+  constexpr uint32_t CH = Gm::CH;
+  extern __shared__ __align__(128) uint8_t smem_ap[];
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint8_t *ring = smem_ap + Gm::RING_OFF + warp * AP_STAGES * Gm::STAGE;
+  float *red = reinterpret_cast<float *>(smem_ap + Gm::RED_OFF), *ml = reinterpret_cast<float *>(smem_ap + Gm::ML_OFF);
+  uint32_t *valid_of = reinterpret_cast<uint32_t *>(smem_ap + Gm::VALID_OFF) + warp * AP_STAGES, *misc = reinterpret_cast<uint32_t *>(smem_ap + Gm::MISC_OFF);
+  uint64_t *misc64 = reinterpret_cast<uint64_t *>(misc);
+  pdl_prologue();
+  const uint32_t units = a.kv.n_kv * a.groups;
+
+  // ---- the share: chunks [x0, x1) of all, and the row it starts in
+  uint32_t per = (a.R + AP_THREADS - 1u) / AP_THREADS, r_lo = min(a.R, tid * per), r_hi = min(a.R, r_lo + per);
+  uint64_t mine = 0u;
+  for (uint32_t r = r_lo; r < r_hi; r++) {
+    uint32_t seq;
+    mine += (ap_row(a, r, seq) + CH - 1u) / CH;
+  }
+  uint64_t incl = mine;
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint64_t v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+    if ((int)lane >= o) incl += v;
+  }
+  if (lane == 31) misc64[warp] = incl;
+  __syncthreads();
+  uint64_t before = incl - mine, all = 0u;
+  for (uint32_t w = 0; w < AP_WARPS; w++) {
+    const uint64_t v = misc64[w];
+    if (w < warp) before += v;
+    all += v;
+  }
+  all *= units, before *= units, mine *= units;
+  uint64_t share = (all + gridDim.x - 1u) / gridDim.x;
+  if (share < a.min_share) share = a.min_share;
+  const uint64_t x0 = min(all, share * blockIdx.x), x1 = min(all, x0 + share);
+  if (x0 < x1 && before <= x0 && x0 < before + mine) {  // one thread
+    uint32_t r = r_lo, seq;
+    uint64_t row;
+    for (;; r++) {
+      row = (uint64_t)((ap_row(a, r, seq) + CH - 1u) / CH) * units;
+      if (x0 < before + row) break;
+      before += row;
+    }
+    misc[8] = r, misc64[5] = x0 - before;  // row, chunk of the row
+  }
+  __syncthreads();
+
+  if (x0 < x1) {
+    ApCursor c;  // what is worked on
+    {
+      c.r = misc[8];
+      c.len = ap_row(a, c.r, c.seq);
+      const uint32_t lc = (c.len + CH - 1u) / CH;
+      const uint64_t at = misc64[5];
+      c.unit = (uint32_t)(at / lc), c.j0 = (uint32_t)(at - (uint64_t)c.unit * lc);
+      c.left = x1 - x0;
+      c.j1 = (uint32_t)min((uint64_t)lc, c.j0 + c.left);
+      c.left -= c.j1 - c.j0;
+    }
+    auto advance = [&](ApCursor &k) {  // to the next unit (k.left > 0: there is one)
+      if (++k.unit == units) {
+        k.unit = 0u;
+        do k.len = ap_row(a, ++k.r, k.seq);
+        while (k.len == 0u);
+      }
+      k.j0 = 0u, k.j1 = (uint32_t)min((uint64_t)((k.len + CH - 1u) / CH), k.left);
+      k.left -= k.j1;
+    };
+
+    // ---- the ring: this warp's chunks, in the order in which they are worked on, AP_STAGES - 1 ahead
+    ApCursor f = c;  // what is fetched
+    uint32_t fj = f.j0 + warp, f_num = 0u, f_stage = 0u;
+    const uint32_t cpp = a.kv.page / CH;
+    bool more = true;
+    auto find = [&] {  // the next chunk of this warp and its page number (needed only one chunk later: nobody waits for it)
+      while (fj >= f.j1) {
+        if (f.left == 0u) {
+          more = false;
+          return;
+        }
+        advance(f);
+        fj = warp;
+      }
+      f_num = page_number(a.kv, f.seq, fj / cpp);
+    };
+    auto fetch = [&] {
+      if (more) {
+        const bool there = f_num < a.kv.n_pages;
+        const uint32_t valid = there ? min(CH, f.len - fj * CH) : 0u;
+        if (!there && a.err && lane == 0) atomicExch(a.err, ERR_PAGES);
+        const size_t from = there ? page_row(a.kv, f_num, f.unit / a.groups, (fj % cpp) * CH, Gm::ROWB) : 0u;
+        const char *ks = static_cast<const char *>(a.kv.kp) + from, *vs = static_cast<const char *>(a.kv.vp) + from;
+        uint8_t *st = ring + f_stage * Gm::STAGE;
+#pragma unroll
+        for (int i = 0; i < Gm::PER_LANE; i++) {
+          const uint32_t n = lane + 32u * i, row = n / Gm::PIECES, piece = n % Gm::PIECES, to = Gm::at(row, piece);
+          const bool in = row < valid;
+          const size_t src = in ? n * 16u : 0u;
+          __pipeline_memcpy_async(st + to, ks + src, 16, in ? 0 : 16);
+          __pipeline_memcpy_async(st + CH * Gm::ROWB + to, vs + src, 16, in ? 0 : 16);
+        }
+        if (lane == 0) valid_of[f_stage] = valid;
+        fj += AP_WARPS;
+        find();
+      }
+      __pipeline_commit();
+      f_stage = f_stage + 1u == AP_STAGES ? 0u : f_stage + 1u;
+    };
+    find();
+#pragma unroll
+    for (int i = 0; i < AP_STAGES - 1; i++) fetch();
+
+    ApWarp<KV, HD> w;
+    uint32_t stage = 0u;
+    uint64_t x = x0;  // global number of chunk c.j0 of the unit
+    while (true) {
+      const uint32_t kvh = c.unit / a.groups, grp = c.unit - kvh * a.groups, h0 = kvh * a.G + grp * a.gw, heads = min(a.gw, a.G - grp * a.gw);
+      const float *q = reinterpret_cast<const float *>(reinterpret_cast<const char *>(a.q) + a.q_stride * c.r) + (size_t)h0 * HD;
+      if (!Gm::F16) {
+        float *qs = reinterpret_cast<float *>(smem_ap + Gm::Q_OFF);  // (the barriers at the end of a unit: nobody reads the last one's any more)
+        for (uint32_t i = tid; i < AP_HEADS * HD; i += AP_THREADS) qs[i] = i < heads * HD ? q[i] : 0.0f;
+        __syncthreads();
+      }
+      w.start(q, heads, smem_ap + Gm::Q_OFF, lane);
+      for (uint32_t j = c.j0 + warp; j < c.j1; j += AP_WARPS) {
+        __pipeline_wait_prior(AP_STAGES - 2);
+        __syncwarp();
+        const uint32_t valid = valid_of[stage];
+        fetch();
+        w.chunk(ring + stage * Gm::STAGE, valid, a.scale_log2, lane);
+        stage = stage + 1u == AP_STAGES ? 0u : stage + 1u;
+      }
+      // ---- the warps' records meet
+      if (!Gm::F16) __syncthreads();  // (q lies where they go)
+      w.finish(red + warp * AP_HEADS * Gm::RED_ROW, ml + warp * AP_HEADS * 2, lane);
+      __syncthreads();
+      const uint32_t lc = (c.len + CH - 1u) / CH;
+      const bool whole = c.j0 == 0u && c.j1 == lc;
+      constexpr uint32_t QUADS = HD / 4, REC = AP_HEADS * Gm::RED_ROW;
+      for (uint32_t i0 = warp * 32u; i0 < heads * QUADS; i0 += AP_THREADS) {
+        const uint32_t i = i0 + lane, h = min(i / QUADS, AP_HEADS - 1u), d = i % QUADS * 4u;
+        float M = -INFINITY, L = 0.0f;
+#pragma unroll
+        for (int k = 0; k < AP_WARPS; k++) M = fmaxf(M, ml[k * AP_HEADS * 2 + 2 * h]);
+        const float base = M == -INFINITY ? 0.0f : M;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < AP_WARPS; k++) {
+          const float f = ex2(ml[k * AP_HEADS * 2 + 2 * h] - base);
+          const float4 v = *reinterpret_cast<const float4 *>(red + k * REC + h * Gm::RED_ROW + d);
+          L = fmaf(f, ml[k * AP_HEADS * 2 + 2 * h + 1], L);
+          acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
+        }
+        const bool in = i < heads * QUADS;
+        if (whole) {
+          const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;  // (a NaN stays one)
+          acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
+          store_row4<HD>(a.out, a.out_stride, a.oq, a.oq_stride, a.wide, a.n_head * HD / 32u, c.r, h0 + h, d, acc, in);
+        } else if (in) {
+          float *to = a.rec + ((size_t)blockIdx.x * 2u + (c.j0 == 0u ? 1u : 0u)) * REC + h * Gm::RED_ROW;
+          *reinterpret_cast<float4 *>(to + d) = acc;
+          if (d == 0u) to[HD] = M, to[HD + 1] = L;
+        }
+      }
+      if (!whole) {
+        // The parts of the unit, in the order of its positions: the second record of the CTA it starts in, then the first ones of the
+        // CTAs behind. Whoever is the last to have written adds them up.
+        const uint64_t u0 = x - c.j0;
+        const uint32_t c0 = (uint32_t)(u0 / share), parts = (uint32_t)((u0 + lc - 1u) / share) - c0 + 1u;
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) {
+          const bool last = atomicAdd(&a.count[c0], 1u) == parts - 1u;
+          if (last) a.count[c0] = 0u;  // left zero for the next launch
+          misc[12] = last;
+        }
+        __syncthreads();
+        if (misc[12]) {
+          __threadfence();
+          for (uint32_t i0 = warp * 32u; i0 < heads * QUADS; i0 += AP_THREADS) {
+            const uint32_t i = i0 + lane, h = min(i / QUADS, heads - 1u), d = i % QUADS * 4u;
+            const float *rec = a.rec + (size_t)c0 * 2u * REC + h * Gm::RED_ROW;
+            auto part = [&](uint32_t k) { return rec + (size_t)(2u * k + (k == 0u ? 1u : 0u)) * REC; };
+            float M = -INFINITY, L = 0.0f;
+            for (uint32_t k = i % QUADS; k < parts; k += QUADS) M = fmaxf(M, __ldcg(part(k) + HD));
+#pragma unroll
+            for (uint32_t o = 1; o < (QUADS < 32u ? QUADS : 32u); o <<= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, o));
+            const float base = M == -INFINITY ? 0.0f : M;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+            for (uint32_t k = 0; k < parts; k++) {
+              const float2 e = __ldcg(reinterpret_cast<const float2 *>(part(k) + HD));
+              const float4 v = __ldcg(reinterpret_cast<const float4 *>(part(k) + d));
+              const float f = ex2(e.x - base);
+              L = fmaf(f, e.y, L);
+              acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
+            }
+            const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
+            acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
+            store_row4<HD>(a.out, a.out_stride, a.oq, a.oq_stride, a.wide, a.n_head * HD / 32u, c.r, h0 + h, d, acc, i < heads * QUADS);
+          }
+        }
+      }
+      x += c.j1 - c.j0;
+      if (c.left == 0u) break;
+      advance(c);
+      __syncthreads();  // everybody has read the records (and misc): the next unit's may be written
+    }
+    __pipeline_wait_prior(0);
+  }
+
+  // ---- rows that see nothing: zeros
+  for (uint32_t r = blockIdx.x; r < a.R; r += gridDim.x) {
+    uint32_t seq;
+    if (ap_row(a, r, seq) != 0u || seq >= a.kv.n_seq) {
+      if (seq < a.kv.n_seq && a.err && tid == 0 && __ldg(a.len + r) > table_positions(a.kv)) atomicExch(a.err, ERR_PAGES);
+      continue;
+    }
+    float *out = reinterpret_cast<float *>(reinterpret_cast<char *>(a.out) + a.out_stride * r);
+    for (uint32_t i = tid; i < a.n_head * HD; i += AP_THREADS) out[i] = 0.0f;
+    if (a.oq)
+      for (uint32_t i = tid; i < a.n_head * HD / 32u * 10u; i += AP_THREADS) reinterpret_cast<uint32_t *>(a.oq + a.oq_stride * r)[i] = 0u;
+  }
+}
+
+constexpr size_t AP_COUNT_BYTES = AP_MAX_CTAS * 4u;
+static size_t ap_record_bytes(uint32_t hd) { return (size_t)AP_HEADS * (hd + 4u) * sizeof(float); }
+
+template <typename KV, int HD>
+static int launch_ap(PagedAttnArgs &a, cudaStream_t st) {
+  using Gm = ApGeom<KV, HD>;
+  auto k = attn_paged_kernel<KV, HD>;
+  if (int r = ensure_dynamic_smem(reinterpret_cast<const void *>(k), Gm::TOTAL)) return r;
+  const uint32_t sms = (uint32_t)sm_count(), ctas = sms * Gm::CTAS < AP_MAX_CTAS ? sms * Gm::CTAS : AP_MAX_CTAS;
+  a.min_share = 256u / Gm::CH;
+  IEB_LAUNCH_PDL("attn_paged_kernel", k, dim3(ctas), dim3(AP_THREADS), Gm::TOTAL, st, a);
+  return IE_B200_OK;
+}
+
+}  // namespace ieb
+
+using namespace ieb;
+
+extern "C" size_t ie_b200_attn_decode_paged_scratch_bytes(uint32_t n_head, uint32_t n_kv, uint32_t hd) {
+  (void)n_head, (void)n_kv;
+  return AP_COUNT_BYTES + (size_t)AP_MAX_CTAS * 2u * ap_record_bytes(hd);
+}
+
+extern "C" int ie_b200_attn_decode_paged(const float *d_q, const ie_b200_kv_pages *pages, float *d_out, void *d_oq, const uint32_t *d_len, const uint32_t *d_seq,
+                                         uint32_t n_head, uint32_t R, size_t q_stride, size_t out_stride, size_t oq_stride, void *d_scratch, uint32_t *d_err,
+                                         void *stream) {
+  if (int r = check_pages("ie_b200_attn_decode_paged", pages, 16u)) return r;
+  if (!d_q || !d_out || !d_len || !d_scratch) return fail(IE_B200_E_ARG, "ie_b200_attn_decode_paged: NULL pointer");
+  if ((((uintptr_t)d_q | q_stride) & 7u) || (((uintptr_t)d_out | out_stride | (uintptr_t)d_oq | oq_stride | (uintptr_t)d_len | (uintptr_t)d_seq) & 3u) || !aligned16(d_scratch))
+    return fail(IE_B200_E_ARG, "ie_b200_attn_decode_paged: alignment (q 8 bytes, outputs 4, scratch 16)");
+  const uint32_t hd = pages->hd, n_kv = pages->n_kv;
+  if (n_head == 0 || n_head % n_kv || n_head > 65535u) return fail(IE_B200_E_SIZE, "ie_b200_attn_decode_paged: %u heads over %u KV heads", n_head, n_kv);
+  if (hd != 32 && hd != 64 && hd != 128) return fail(IE_B200_E_SIZE, "ie_b200_attn_decode_paged: head dim %u unsupported (32, 64, 128)", hd);
+  if (R == 0) return IE_B200_OK;
+  const size_t row = (size_t)n_head * hd;
+  if (R > (1u << 20) || (R > 1u && (q_stride < row * 4u || out_stride < row * 4u || (d_oq && oq_stride < row / 32u * 40u))))
+    return fail(IE_B200_E_SIZE, "ie_b200_attn_decode_paged: %u rows (at most 2^20) with strides of %zu, %zu and %zu bytes", R, q_stride, out_stride, oq_stride);
+  PagedAttnArgs a = {};
+  a.q = d_q, a.out = d_out, a.oq = static_cast<uint8_t *>(d_oq), a.len = d_len, a.seq = d_seq, a.err = d_err, a.kv = *pages;
+  a.count = static_cast<uint32_t *>(d_scratch), a.rec = reinterpret_cast<float *>(static_cast<char *>(d_scratch) + AP_COUNT_BYTES);
+  a.n_head = n_head, a.G = n_head / n_kv, a.groups = (a.G + AP_HEADS - 1u) / AP_HEADS, a.gw = (a.G + a.groups - 1u) / a.groups, a.R = R;
+  a.wide = (((uintptr_t)d_out | out_stride) & 15u) == 0u;
+  a.q_stride = q_stride, a.out_stride = out_stride, a.oq_stride = oq_stride;
+  a.scale_log2 = 1.44269504088896340736f / sqrtf((float)hd);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (pages->kv_f32) return hd == 32 ? launch_ap<float, 32>(a, st) : hd == 64 ? launch_ap<float, 64>(a, st) : launch_ap<float, 128>(a, st);
+  return hd == 32 ? launch_ap<__half, 32>(a, st) : hd == 64 ? launch_ap<__half, 64>(a, st) : launch_ap<__half, 128>(a, st);
+}

@@ -39,6 +39,7 @@
 #include <algorithm>
 
 #include "attn_prefill_tc.cuh"
+#include "row_store.cuh"
 #include "tc_common.cuh"
 
 namespace ieb {
@@ -61,12 +62,6 @@ struct PtArgs {
   const __half *vc;  // the V cache (read here only for rows that hold an infinity or a NaN)
 };
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // Eight neighbouring floats of a row: one 32-byte access (whole sectors, however far apart the lanes' rows lie) where aligned.
 __device__ __forceinline__ void ld8(const float *p, float (&x)[8], bool wide) {
   if (wide) {
@@ -86,38 +81,6 @@ __device__ __forceinline__ void st8(float *p, const uint32_t *v, bool wide) {
     for (int e = 0; e < 8; e++) p[e] = __uint_as_float(v[e]);
   }
 }
-
-// Four neighbouring outputs of a (token, head) row per lane, eight lanes per block of 32: the row's floats and its Q8 copy.
-template <int HD>
-__device__ __forceinline__ void store_row4(float *out, size_t out_stride, uint8_t *oq, size_t oq_stride, uint32_t wide, uint32_t nbq, uint32_t tok, uint32_t head,
-                                           uint32_t col, const float4 &o, bool in) {
-  float *dst = reinterpret_cast<float *>(reinterpret_cast<char *>(out) + out_stride * tok) + (size_t)head * HD + col;
-  if (in) {
-    if (wide) *reinterpret_cast<float4 *>(dst) = o;
-    else dst[0] = o.x, dst[1] = o.y, dst[2] = o.z, dst[3] = o.w;
-  }
-  if (!oq) return;
-  float amax = fmaxf(fmaxf(fabsf(o.x), fabsf(o.y)), fmaxf(fabsf(o.z), fabsf(o.w)));
-#pragma unroll
-  for (int s = 1; s < 8; s <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, s));
-  const float d = __fdiv_rn(amax, 127.0f), v[4] = {o.x, o.y, o.z, o.w};
-  const Q8Div qd = q8_div(d);
-  int sum = 0;
-  uint32_t w = 0u;
-#pragma unroll
-  for (int e = 0; e < 4; e++) {
-    const int q = q8_round(v[e], qd);
-    sum += q, w |= (uint32_t)(q & 255) << (8 * e);
-  }
-#pragma unroll
-  for (int s = 1; s < 8; s <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, s);
-  if (!in) return;
-  uint8_t *qrow = oq + oq_stride * tok;
-  const uint32_t at = head * HD + col;
-  *reinterpret_cast<uint32_t *>(qrow + at) = w;
-  if ((at & 31u) == 0u) reinterpret_cast<float *>(qrow + 32u * (size_t)nbq)[at / 32u] = d, reinterpret_cast<int *>(qrow + 36u * (size_t)nbq)[at / 32u] = sum;
-}
-
 
 // r / G for r below 2^22 (exact: r + 0.5 is at least 0.5 / G away from a multiple of G, the product's error below 2^-23 of it)
 __device__ __forceinline__ uint32_t row_token(uint32_t r, float inv_g) { return (uint32_t)(((float)r + 0.5f) * inv_g); }

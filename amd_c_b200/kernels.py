@@ -293,3 +293,120 @@ def argmax(x: torch.Tensor) -> torch.Tensor:
     out = torch.empty((T, 2), dtype=torch.int32, device=x.device)
     check(lib.ie_b200_argmax(x2.data_ptr(), n, out.data_ptr(), T, x2.stride(0) * 4, 8, part.data_ptr(), _stream()))
     return out
+
+
+# ---- many sequences: a paged KV cache, attention over it, the draw of the next tokens. These take tensors of a server's own
+# making, so they look at them first; the work goes to the tensors' device, on its current stream. A decode step of one token is host
+# time, so what is usual is passed by one expression per tensor and only what fails it is looked at closely.
+def _refuse(name: str, t, dtype, shape, dev: int, what: str) -> None:
+    got = f"{t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
+    raise ValueError(f"{name}: want {dtype} {tuple('any' if n is None else n for n in shape)} on cuda:{dev}, {what}; got {got}")
+
+
+def _flat(name: str, t: torch.Tensor, dtype, shape: tuple, dev: int) -> int:
+    """The address of a contiguous tensor of that type and shape on GPU `dev`."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != dev or t.shape != shape or not t.is_contiguous():
+        _refuse(name, t, dtype, shape, dev, "contiguous")
+    return t.data_ptr()
+
+
+def _rows(name: str, t: torch.Tensor, dtype, n: int | None, cols: int | None, dev: int) -> tuple[int, int, int, int]:
+    """(address, rows, columns, elements from row to row) of a 2-D tensor whose rows are contiguous and do not overlap; n, cols: what
+    it has to have (None: any)."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == dev and t.dim() == 2:
+        rows, width = t.shape
+        step, by = t.stride()
+        if rows <= 1:
+            step = width
+        if (n is None or rows == n) and (cols is None or width == cols) and (by == 1 or width <= 1) and step >= width:
+            return t.data_ptr(), rows, width, step
+    _refuse(name, t, dtype, (n, cols), dev, "rows contiguous and apart")
+
+
+def _kv_pages(kp: torch.Tensor, vp: torch.Tensor, table: torch.Tensor) -> tuple[bytes, int, int, int, int]:
+    """ie_b200_kv_pages of kp / vp [n_pages, n_kv, page, hd] half or float, pages any distance apart (alike in both), and a table
+    [n_seq, columns] int32; with it the GPU, KV heads, head size and sequences."""
+    if not isinstance(kp, torch.Tensor) or kp.dim() != 4 or not kp.is_cuda or kp.dtype not in (torch.half, torch.float):
+        raise ValueError("kp: want a half or float CUDA tensor [n_pages, n_kv, page, hd]")
+    dev, dtype, shape, strides = kp.get_device(), kp.dtype, kp.shape, kp.stride()
+    n, n_kv, page, hd = shape
+    own = page * hd
+    if (strides[1:] != (own, hd, 1) or not isinstance(vp, torch.Tensor) or vp.stride() != strides or vp.shape != shape or vp.dtype is not dtype
+            or vp.get_device() != dev):
+        for name, x in (("kp", kp), ("vp", vp)):  # (sizes of one, and a single page, have any stride)
+            if not isinstance(x, torch.Tensor) or x.dtype is not dtype or x.get_device() != dev or x.shape != shape or not n or not x[0].is_contiguous() or (
+                    n > 1 and x.stride(0) != strides[0]):
+                _refuse(name, x, dtype, shape, dev, "each page contiguous, the pages of both as far apart")
+    size = 4 if dtype is torch.float else 2
+    at, n_seq, cols, stride = _rows("table", table, torch.int32, None, None, dev)
+    return (_lib.KV_PAGES.pack(kp.data_ptr(), vp.data_ptr(), at, n, page, n_kv, hd, n_seq, cols, stride, size == 4, (strides[0] if n > 1 else n_kv * own) * size),
+            dev, n_kv, hd, n_seq)
+
+
+def _launch(fn, dev: int, *args) -> None:
+    """fn(*args, stream) on GPU dev and its current stream."""
+    if dev == torch.cuda.current_device():
+        check(fn(*args, torch._C._cuda_getCurrentRawStream(dev)))
+    else:
+        with torch.cuda.device(dev):
+            check(fn(*args, torch._C._cuda_getCurrentRawStream(dev)))
+
+
+def _seq(seq: torch.Tensor | None, n: int, n_seq: int, dev: int) -> int | None:
+    if seq is not None:
+        return _flat("seq", seq, torch.int32, (n,), dev)
+    if n > n_seq:
+        raise ValueError(f"{n} rows of their own sequences against a table of {n_seq}")
+    return None
+
+
+def _err(err: torch.Tensor | None, dev: int) -> int | None:
+    return None if err is None else _flat("err", err, torch.int32, (1,), dev)
+
+
+def rope_kv_paged(qkv: torch.Tensor, kp: torch.Tensor, vp: torch.Tensor, table: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: torch.Tensor,
+                  seq: torch.Tensor | None, nq: int, nkv: int, hd: int, neox: bool, out: torch.Tensor | None = None, err: torch.Tensor | None = None) -> torch.Tensor:
+    """New tokens of many sequences: qkv [T, (nq + 2 nkv) hd] f32 un-rotated (not changed); token t is position pos[t] of sequence
+    seq[t] (None: of sequence t). Stores the rotated k and v into the pages and returns the rotated q [T, nq hd] (in `out` if given).
+    A seq[t] of n_seq or more (-1 too) marks a token that only pads the batch: nothing is done for it."""
+    pages, dev, kv_heads, kv_hd, n_seq = _kv_pages(kp, vp, table)
+    if nkv != kv_heads or hd != kv_hd:
+        raise ValueError(f"{nkv} KV heads of {hd} against pools of {kv_heads} heads of {kv_hd}")
+    base, T, _, step = _rows("qkv", qkv, torch.float, None, (nq + 2 * nkv) * hd, dev)
+    c, n_rope, half, row = _rows("cos", cos, torch.float, None, hd // 2, dev)
+    if row != half:
+        _refuse("cos", cos, torch.float, (None, half), dev, "contiguous")
+    if out is None:
+        out = torch.empty((T, nq * hd), dtype=torch.float32, device=qkv.device)
+    to, _, _, out_step = _rows("out", out, torch.float, T, nq * hd, dev)
+    _launch(_lib.load().ie_b200_rope_kv_paged, dev, base, base + 4 * nq * hd, base + 4 * (nq + nkv) * hd, to, pages, c,
+            _flat("sin", sin, torch.float, (n_rope, half), dev), n_rope, _flat("pos", pos, torch.int32, (T,), dev), _seq(seq, T, n_seq, dev), nq,
+            1 if neox else 0, T, step * 4, out_step * 4, _err(err, dev))
+    return out
+
+
+class PagedScratch:
+    """Counters and partial records of attn_decode_paged for one head layout, on one device. One call at a time may use it."""
+
+    def __init__(self, n_head: int, n_kv: int, hd: int, device):
+        self.data = torch.zeros(_lib.load().ie_b200_attn_decode_paged_scratch_bytes(n_head, n_kv, hd), dtype=torch.uint8, device=device)
+        self.layout = (n_head, n_kv, hd)
+
+
+def attn_decode_paged(q: torch.Tensor, kp: torch.Tensor, vp: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, n_head: int, scratch: PagedScratch,
+                      seq: torch.Tensor | None = None, quant: bool = True, out: torch.Tensor | None = None, err: torch.Tensor | None = None):
+    """One query token per row: q [R, n_head hd] f32 (rotated), row r sees the first lens[r] positions of sequence seq[r] (None: of
+    sequence r). Returns (out [R, n_head hd], Q8 copies or None); a row that sees nothing is zeros, a row whose seq[r] is n_seq or
+    more (-1 too) is left as it was."""
+    pages, dev, n_kv, hd, n_seq = _kv_pages(kp, vp, table)
+    at, R, _, step = _rows("q", q, torch.float, None, n_head * hd, dev)
+    if scratch.layout != (n_head, n_kv, hd) or scratch.data.get_device() != dev:
+        raise ValueError(f"scratch for {scratch.layout} (heads, KV heads, head size) on {scratch.data.device}, not {(n_head, n_kv, hd)} on cuda:{dev}")
+    if out is None:
+        out = torch.empty((R, n_head * hd), dtype=torch.float32, device=q.device)
+    to, _, _, out_step = _rows("out", out, torch.float, R, n_head * hd, dev)
+    nbq = n_head * hd // 32
+    oq = torch.empty((R, q8_bytes(nbq)), dtype=torch.uint8, device=q.device) if quant else None
+    _launch(_lib.load().ie_b200_attn_decode_paged, dev, at, pages, to, _p(oq), _flat("lens", lens, torch.int32, (R,), dev), _seq(seq, R, n_seq, dev), n_head, R,
+            step * 4, out_step * 4, q8_bytes(nbq), scratch.data.data_ptr(), _err(err, dev))
+    return out, oq

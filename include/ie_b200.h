@@ -250,6 +250,46 @@ int ie_b200_attn_prefill_split(const float *d_q, const void *d_kc, const void *d
                                uint32_t n_head, uint32_t n_kv, uint32_t hd, uint32_t kv_len, uint32_t T, size_t q_stride, size_t out_stride,
                                size_t oq_stride, uint32_t positions, void *d_scratch, uint32_t *d_err, void *stream);
 
+/* -------------------------------------------------- paged KV cache (many sequences)
+ * Two pools of pages, K and V alike: [n_pages][n_kv][page][hd] of half (kv_f32 0) or float (1) elements, consecutive pages
+ * page_stride bytes apart (a pool may interleave layers, or K and V). Position p of sequence s lies in row p % page of the
+ * page whose number is table[s * table_stride + p / page]; the pages of a sequence may lie anywhere and may be shared
+ * between sequences. The reference keeps one contiguous cache for its one sequence (src/plan.c; ie_rope_kv and ie_attn_kv,
+ * src/hip.c:1284, :1492) and has no counterpart of this.
+ * What the device arrays hold is checked on the device: a sequence number of n_seq or more marks a row that only pads the
+ * batch (its outputs are left as they were); a position outside the table, or on a page whose number is n_pages or more, does not exist:
+ * nothing is stored for it, attention leaves it out, and *d_err (may be NULL) is set to 6. */
+typedef struct {
+  void *kp, *vp;               /* device pools, 16-byte aligned */
+  const uint32_t *table;       /* device, [n_seq][table_stride] page numbers, table_cols of them valid */
+  uint32_t n_pages, page, n_kv, hd, n_seq, table_cols, table_stride;
+  int kv_f32;
+  size_t page_stride;          /* bytes, a multiple of 16 */
+} ie_b200_kv_pages;
+
+/* RoPE of T new tokens and the store of their K / V rows into the pages: token t is position d_pos[t] of sequence d_seq[t]
+ * (d_seq NULL: of sequence t). The rotated q goes to d_q_out (nq heads, rows q_out_stride bytes apart; it may be d_q itself
+ * with the same stride), k is rotated and stored with v, neither is written back. Same bits as ie_b200_rope_kv; d_cos / d_sin:
+ * n_rope rows of hd / 2 floats (a position past them counts as outside the table; such a token's q_out row is left as it was).
+ * nq may be 0 (d_q, d_q_out unused). The tokens of a call name different positions: of two that name the same row of the
+ * same page either may end up there, or a part of each. hd: a multiple of 8 up to 512; any page size; strides in bytes. */
+int ie_b200_rope_kv_paged(const float *d_q, const float *d_k, const float *d_v, float *d_q_out, const ie_b200_kv_pages *pages, const float *d_cos,
+                          const float *d_sin, uint32_t n_rope, const uint32_t *d_pos, const uint32_t *d_seq, uint32_t nq, int neox, uint32_t T,
+                          size_t qkv_stride, size_t q_out_stride, uint32_t *d_err, void *stream);
+
+/* Attention of R rows, one query token each, over the pages: row r sees positions 0 .. d_len[r] - 1 of sequence d_seq[r]
+ * (d_seq NULL: of sequence r). Several rows may name one sequence (the tokens of a prompt, of a draft). A row that sees
+ * nothing (length 0) is zeros. The work is dealt out evenly over the GPU whatever the lengths are; where it cuts a (row, KV
+ * head) into parts the last part to finish merges them, in a fixed order. The result of a row does not depend on the bits
+ * of rows it does not see. Optional Q8 copies of the rows (d_oq). hd 32, 64 or 128, n_head a multiple of n_kv, pages of a multiple of 16 positions;
+ * q 8-byte aligned, strides in bytes. d_scratch: ie_b200_attn_decode_paged_scratch_bytes() bytes of the device the call is
+ * made on, 16-byte aligned, zero before the first call and left ready by every call; calls that share it (graphs that
+ * captured them too) must not overlap on the GPU. */
+size_t ie_b200_attn_decode_paged_scratch_bytes(uint32_t n_head, uint32_t n_kv, uint32_t hd);
+int ie_b200_attn_decode_paged(const float *d_q, const ie_b200_kv_pages *pages, float *d_out, void *d_oq, const uint32_t *d_len, const uint32_t *d_seq,
+                              uint32_t n_head, uint32_t R, size_t q_stride, size_t out_stride, size_t oq_stride, void *d_scratch, uint32_t *d_err,
+                              void *stream);
+
 /* First index of the maximum of each of T rows, and the softmax probability
  * of that maximum: OP_ARGMAX (src/cpu.c:608-614), ie_argmax
  * {x,n,out,part,count,ng} (src/hip.c:1537). out: {u32 index, f32 prob} per row.
