@@ -533,6 +533,7 @@ extern "C" size_t ie_b200_attn_decode_paged_scratch_bytes(uint32_t n_head, uint3
 extern "C" int ie_b200_attn_decode_paged(const float *d_q, const ie_b200_kv_pages *pages, float *d_out, void *d_oq, const uint32_t *d_len, const uint32_t *d_seq,
                                          uint32_t n_head, uint32_t R, size_t q_stride, size_t out_stride, size_t oq_stride, void *d_scratch, uint32_t *d_err,
                                          void *stream) {
+  if (R == 0) return IE_B200_OK;  // (an empty tensor may have no address)
   if (int r = check_pages("ie_b200_attn_decode_paged", pages, 16u)) return r;
   if (!d_q || !d_out || !d_len || !d_scratch) return fail(IE_B200_E_ARG, "ie_b200_attn_decode_paged: NULL pointer");
   if ((((uintptr_t)d_q | q_stride) & 7u) || (((uintptr_t)d_out | out_stride | (uintptr_t)d_oq | oq_stride | (uintptr_t)d_len | (uintptr_t)d_seq) & 3u) || !aligned16(d_scratch))
@@ -540,7 +541,6 @@ extern "C" int ie_b200_attn_decode_paged(const float *d_q, const ie_b200_kv_page
   const uint32_t hd = pages->hd, n_kv = pages->n_kv;
   if (n_head == 0 || n_head % n_kv || n_head > 65535u) return fail(IE_B200_E_SIZE, "ie_b200_attn_decode_paged: %u heads over %u KV heads", n_head, n_kv);
   if (hd != 32 && hd != 64 && hd != 128) return fail(IE_B200_E_SIZE, "ie_b200_attn_decode_paged: head dim %u unsupported (32, 64, 128)", hd);
-  if (R == 0) return IE_B200_OK;
   const size_t row = (size_t)n_head * hd;
   if (R > (1u << 20) || (R > 1u && (q_stride < row * 4u || out_stride < row * 4u || (d_oq && oq_stride < row / 32u * 40u))))
     return fail(IE_B200_E_SIZE, "ie_b200_attn_decode_paged: %u rows (at most 2^20) with strides of %zu, %zu and %zu bytes", R, q_stride, out_stride, oq_stride);

@@ -130,12 +130,12 @@ using namespace ieb;
 extern "C" int ie_b200_rope_kv_paged(const float *d_q, const float *d_k, const float *d_v, float *d_q_out, const ie_b200_kv_pages *pages, const float *d_cos,
                                      const float *d_sin, uint32_t n_rope, const uint32_t *d_pos, const uint32_t *d_seq, uint32_t nq, int neox, uint32_t T,
                                      size_t qkv_stride, size_t q_out_stride, uint32_t *d_err, void *stream) {
+  if (T == 0) return IE_B200_OK;  // (an empty tensor may have no address)
   if (int r = check_pages("ie_b200_rope_kv_paged", pages, 1u)) return r;
   if ((nq && (!d_q || !d_q_out)) || !d_k || !d_v || !d_cos || !d_sin || !d_pos) return fail(IE_B200_E_ARG, "ie_b200_rope_kv_paged: NULL pointer");
   if (((uintptr_t)d_q | (uintptr_t)d_k | (uintptr_t)d_v | (uintptr_t)d_q_out | (uintptr_t)d_cos | (uintptr_t)d_sin | (uintptr_t)d_pos | (uintptr_t)d_seq | qkv_stride | q_out_stride) & 3u)
     return fail(IE_B200_E_ARG, "ie_b200_rope_kv_paged: pointers and strides must be 4-byte aligned");
   if (nq > 65535u) return fail(IE_B200_E_SIZE, "ie_b200_rope_kv_paged: %u query heads", nq);
-  if (T == 0) return IE_B200_OK;
   if (T > 0x7FFFFFFFu || (T > 1u && (qkv_stride < (size_t)pages->n_kv * pages->hd * 4u || (nq && q_out_stride < (size_t)nq * pages->hd * 4u))))
     return fail(IE_B200_E_SIZE, "ie_b200_rope_kv_paged: %u tokens with rows %zu and %zu bytes apart", T, qkv_stride, q_out_stride);
   RopePagedArgs a = {d_q, d_k, d_v, d_cos, d_sin, d_q_out, d_pos, d_seq, d_err, *pages, nq, n_rope, qkv_stride, q_out_stride};

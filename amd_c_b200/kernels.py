@@ -410,3 +410,21 @@ def attn_decode_paged(q: torch.Tensor, kp: torch.Tensor, vp: torch.Tensor, table
     _launch(_lib.load().ie_b200_attn_decode_paged, dev, at, pages, to, _p(oq), _flat("lens", lens, torch.int32, (R,), dev), _seq(seq, R, n_seq, dev), n_head, R,
             step * 4, out_step * 4, q8_bytes(nbq), scratch.data.data_ptr(), _err(err, dev))
     return out, oq
+
+
+def sample(x: torch.Tensor, u: torch.Tensor, temp: torch.Tensor | None = None, top_k: torch.Tensor | None = None, top_p: torch.Tensor | None = None,
+           min_p: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The next token of each row of logits x [T, n] f32, drawn with the uniform numbers u [T] f32: (indices int32 [T], probabilities f32
+    [T]). temp, top_p, min_p f32 [T] and top_k int32 [T] are each row's settings; None: 1, 1, 0, 0 (that filter off). A row
+    without a finite logit gives -1 and 0."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise ValueError("x: want a CUDA tensor [T, n]")
+    dev = x.get_device()
+    at, T, n, step = _rows("x", x, torch.float, None, None, dev)
+    row = (T,)
+    out = torch.empty((T, 2), dtype=torch.int32, device=x.device)
+    _launch(_lib.load().ie_b200_sample, dev, at, n, out.data_ptr(), _flat("u", u, torch.float, row, dev),
+            None if temp is None else _flat("temp", temp, torch.float, row, dev), None if top_k is None else _flat("top_k", top_k, torch.int32, row, dev),
+            None if top_p is None else _flat("top_p", top_p, torch.float, row, dev), None if min_p is None else _flat("min_p", min_p, torch.float, row, dev),
+            T, step * 4, 8)
+    return out[:, 0], out.view(torch.float32)[:, 1]

@@ -329,4 +329,5 @@ def test_paged_wrappers_refuse(cuda):
     for bad in (dict(qkv=qkv[:, 1:]), dict(cos=cos[:, 1:]), dict(sin=sin[1:]), dict(pos=n.long()), dict(nkv=4, nq=0), dict(out=qkv), dict(seq=torch.cat([n, n]))):
         with pytest.raises((ValueError, AttributeError)):
             K.rope_kv_paged(**{**dict(qkv=qkv, kp=kp, vp=vp, table=table, cos=cos, sin=sin, pos=n, seq=None, nq=4, nkv=2, hd=64, neox=True), **bad})
-    K.attn_decode_paged(q, kp, vp, table, n, 4, sc)
+    assert K.attn_decode_paged(q[:0], kp, vp, table, n[:0], 4, sc)[0].shape == (0, 256)
+    assert K.rope_kv_paged(qkv[:0], kp, vp, table, cos, sin, n[:0], n[:0], 4, 2, 64, True).shape == (0, 256)
