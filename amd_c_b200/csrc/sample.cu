@@ -7,25 +7,27 @@
 // A draw goes by which side of a sum a number falls, and a row has 10^5 such borders; sums that are off by 1e-7 would move a border
 // past u once in some hundred draws. So weights are fixed-point integers, 2^F for the largest, F = 62 - log2 of the row's length (44 for 2^18
 // tokens): their sums are exact and the same in any order, each weight is off by at most half a unit and the error of the exponential
-// (2^-50: double, a table of 2^(j/64) and a polynomial of degree 5).
+// (2^-49: double, a table of 2^(j/128) and a polynomial of degree 4).
 //
 // One thread-block cluster per row, each CTA with its slice of the row in shared memory: the logits are read from HBM once, all
-// further passes stay on chip, and what the CTAs find meets in each other's shared memory. Bound: 4 bytes per logit for many
-// rows; for few the chain of passes and cluster barriers.
-//  - top-k up to 1024: with j = ceil(k / CTAs), the j-th largest of the 512 threads' own maxima (rounded down to a bin of a histogram of
-//    their leading bits) is a lower bound of each CTA; the smallest of the CTAs' is one for the row: at least k tokens reach it, and few
-//    more. They go to the first CTA, which sorts them and does the rest alone.
-//  - everything else: the border of a run (by count or by mass) from a histogram over the cluster, 2048 bins of 1/64 of a power of two of
-//    the weight, whose bin on the border is sorted by the first CTA, or, where it holds too many, split further by the bits of the
-//    logits until what is left are equal ones; those are counted off by index.
-#include <float.h>
+// further passes stay on chip, and what the CTAs find meets in each other's shared memory. A thread has a contiguous run of tokens, so that
+// sums over threads are sums in index order. Bound: the chain of passes and cluster barriers (some 1000 cycles each; a row takes
+// one to six of them), for many rows also the exponentials of those that need all of them.
+//  - top-k up to 512: the row's 512 groups of threads exchange their maxima; the k-th largest of those (but for its low bits) is a lower
+//    bound: at least k tokens reach it, and few more. They go to the first CTA, which ranks them and does the rest alone.
+//  - everything else: the border of a run (by count or by mass) from a histogram over the cluster, bins of 1/48 of a power of two of
+//    the weight. A bin's mass is two 32-bit words, the upper touched by a carry or a weight of more than 2^32 units only (64-bit
+//    atomics took 150 us at 1 x 128256, 720 at 64 x 152064). A short run of top-p goes to the first CTA whole, as above; of a long one
+//    the bin on the border does, or, where that holds too many, is split further by the bits of the logits until what is left are
+//    equal ones, which are counted off by index.
+#include <cuda_pipeline_primitives.h>
 #include <math.h>
 
 #include "common.cuh"
 
 namespace ieb {
 
-constexpr int SM_THREADS = 512, SM_WARPS = SM_THREADS / 32, SM_BINS = 2048, SM_LIST = 1024, SM_MAX_CL = 8;
+constexpr int SM_THREADS = 512, SM_WARPS = SM_THREADS / 32, SM_PER = 3, SM_BINS = SM_PER * SM_THREADS, SM_LIST = 1024, SM_SHORT = 256, SM_MAX_CL = 8, SM_TABLE = 128;
 constexpr uint32_t SM_MAX_SLICE = 45056;  // floats of a CTA's slice: 176 KB
 constexpr uint32_t SM_NONE = 0xFFFFFFFFu;
 
@@ -38,22 +40,30 @@ struct SampleArgs {
   size_t x_stride, out_stride;
 };
 
-// A CTA's shared memory in front of its slice.
+// A CTA's shared memory in front of its slice (with the slice of 152064 logits over 8 CTAs: two CTAs on an SM).
 struct SampleSmem {
-  uint64_t hist[SM_BINS];            // masses (or counts) of the bins; as u32: counts of the threads' maxima
-  uint64_t list[SM_LIST];            // (key, ~index) of the row's candidates (first CTA)
-  uint64_t mine[SM_LIST];            // this CTA's candidates
-  uint64_t range[SM_MAX_CL];         // masses of the CTAs' ranges of bins, or of their slices
-  uint64_t wsum[2 * SM_WARPS + 2];   // of the warps
-  double pow2[64];                   // 2^(F + j / 64)
-  float max_v[SM_MAX_CL];
-  uint32_t max_i[SM_MAX_CL], floor_key[SM_MAX_CL];
+  uint32_t low[SM_BINS], high[SM_BINS];  // this CTA's histogram
+  union {
+    uint64_t bins[SM_BINS];              // the cluster's
+    struct {
+      uint64_t mine[SM_LIST];            // this CTA's candidates (key, ~index); in the first CTA then the sorted ones of the row
+      uint64_t w[SM_THREADS];            // their weights
+    };
+  };
+  uint64_t list[SM_LIST];                // the row's candidates (first CTA)
+  uint64_t part[SM_MAX_CL];              // sums of the CTAs
+  uint64_t wsum[SM_WARPS];               // of the warps
+  double pow2[SM_TABLE];                 // 2^(F + j / 128)
+  float max_of[SM_THREADS];              // maxima of the row's 512 groups of threads
+  uint32_t first[SM_MAX_CL];             // index of each CTA's maximum
   uint32_t n_list, n_mine, base, bin;
-  uint64_t above;
-  uint32_t cut_key, cut_idx;
+  uint64_t above, cut;                   // mass ahead of the bin; a new cut: key, ~index
 };
+extern __shared__ __align__(16) uint8_t smem_s[];  // SampleSmem, then the slice
+constexpr size_t SM_FRONT = (sizeof(SampleSmem) + 15u) & ~(size_t)15u;
+__device__ __forceinline__ SampleSmem &sm_front() { return *reinterpret_cast<SampleSmem *>(smem_s); }
 
-// Floats in an order of unsigned integers; NaN has been taken for -inf.
+// Floats in an order of unsigned integers.
 __device__ __forceinline__ uint32_t sm_key(float x) {
   const uint32_t b = __float_as_uint(x + 0.0f);  // (-0 is 0)
   return b & 0x80000000u ? ~b : b | 0x80000000u;
@@ -62,9 +72,9 @@ __device__ __forceinline__ float sm_unkey(uint32_t k) { return __uint_as_float(k
 
 __device__ __forceinline__ void dsm_st64(uint32_t a, uint64_t v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory"); }
 __device__ __forceinline__ void dsm_st32(uint32_t a, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory"); }
-__device__ __forceinline__ uint64_t dsm_ld64(uint32_t a) {
-  uint64_t v;
-  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
+__device__ __forceinline__ uint32_t dsm_ld32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
   return v;
 }
 __device__ __forceinline__ uint32_t dsm_add32(uint32_t a, uint32_t v) {
@@ -73,104 +83,217 @@ __device__ __forceinline__ uint32_t dsm_add32(uint32_t a, uint32_t v) {
   return old;
 }
 
-__device__ __forceinline__ uint64_t warp_sum64(uint64_t v) {
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-  return v;
-}
-__device__ __forceinline__ uint64_t warp_scan64(uint64_t v, int lane) {  // inclusive
-  for (int o = 1; o < 32; o <<= 1) {
+__device__ __forceinline__ uint64_t warp_scan64(uint64_t v, uint32_t lane) {  // inclusive
+  for (uint32_t o = 1; o < 32u; o <<= 1) {
     const uint64_t w = __shfl_up_sync(0xFFFFFFFFu, v, o);
     if (lane >= o) v += w;
   }
   return v;
 }
+// The sum of v over the CTA's threads ahead of this one (x), and of all of them (y). (Out of line: it is used in many places.)
+__device__ __noinline__ ulonglong2 sm_before(uint64_t v, uint32_t tid) {
+  SampleSmem &s = sm_front();
+  const uint32_t warp = tid >> 5, lane = tid & 31u;
+  const uint64_t incl = warp_scan64(v, lane);
+  __syncthreads();
+  if (lane == 31u) s.wsum[warp] = incl;
+  __syncthreads();
+  const uint64_t of_warp = lane < SM_WARPS ? s.wsum[lane] : 0u, scan = warp_scan64(of_warp, lane);
+  return make_ulonglong2(__shfl_sync(0xFFFFFFFFu, scan - of_warp, warp) + incl - v, __shfl_sync(0xFFFFFFFFu, scan, 31));
+}
+
+// 2^F w as an integer: t = (x - max) 128 log2(e) / temp = k + f, k the nearest integer, w = 2^(k / 128) 2^(f / 128), each step for all N, so that
+// they run together: a row of which every weight is wanted is bound by the number of instructions, some 25 for each.
+template <int N>
+__device__ __forceinline__ void sm_weights(const double (&diff)[N], double c128, uint64_t (&w)[N]) {
+  constexpr double MAGIC = 6755399441055744.0, L = 0.0054152123481245725;  // 1.5 * 2^52; ln 2 / 128
+  double m[N], f[N], p[N];
+#pragma unroll
+  for (int e = 0; e < N; e++) m[e] = fma(diff[e], c128, MAGIC);  // k in the low bits
+#pragma unroll
+  for (int e = 0; e < N; e++) f[e] = fma(diff[e], c128, MAGIC - m[e]);
+#pragma unroll
+  for (int e = 0; e < N; e++) p[e] = fma(f[e], L * L * L * L / 24.0, L * L * L / 6.0);
+#pragma unroll
+  for (int e = 0; e < N; e++) p[e] = fma(f[e], p[e], L * L / 2.0);
+#pragma unroll
+  for (int e = 0; e < N; e++) p[e] = fma(f[e], p[e], L);
+#pragma unroll
+  for (int e = 0; e < N; e++) p[e] = fma(f[e], p[e], 1.0);
+#pragma unroll
+  for (int e = 0; e < N; e++) p[e] *= sm_front().pow2[__double2loint(m[e]) & (SM_TABLE - 1)];
+#pragma unroll
+  for (int e = 0; e < N; e++)  // (2^52 more: rounded to an integer, in the low bits)
+    p[e] = __hiloint2double(__double2hiint(p[e]) + ((__double2loint(m[e]) & -SM_TABLE) << 13), __double2loint(p[e])) + 4503599627370496.0;
+#pragma unroll
+  for (int e = 0; e < N; e++) w[e] = (uint64_t)__double_as_longlong(p[e]) & 0xFFFFFFFFFFFFFull;
+}
+__device__ __noinline__ uint64_t sm_weight(double diff, double c128) {
+  const double d[1] = {diff};
+  uint64_t w[1];
+  sm_weights<1>(d, c128, w);
+  return w[0];
+}
+
+__device__ __forceinline__ void sample_out(const SampleArgs &a, uint32_t row, uint32_t idx, float prob) {
+  uint32_t *o = reinterpret_cast<uint32_t *>(reinterpret_cast<char *>(a.out) + a.out_stride * row);
+  o[0] = idx, o[1] = __float_as_uint(prob);
+}
+// What a running sum of integers has to exceed to exceed u times the sum, and what it has to reach to reach p times the sum.
+__device__ __forceinline__ uint64_t sample_goal(float u, uint64_t all) {
+  const double g = (double)u * (double)all;
+  return g > 0.0 ? min((uint64_t)min(g, 9.2e18), all - 1u) : 0u;
+}
+__device__ __forceinline__ uint64_t run_goal(float p, uint64_t all) {
+  const double g = ceil((double)p * (double)all);
+  return g > 1.0 ? min(all, (uint64_t)g) : 1u;
+}
 
 struct Sampler {
   const SampleArgs &a;
   SampleSmem &s;
-  float *xs;  // the slice
-  uint32_t rank, cl, begin, count;  // of the cluster; first token and tokens of the slice
-  float xmax, c32;                  // c32: log2(e) / temp
-  double c64, min_w;                // 64 log2(e) / temp; min_p in units of the weights
-  float far;                        // log2 distance from which a weight is not needed (0, or below min_p)
-  uint32_t tid, warp, lane;
+  float *xs;                             // the slice
+  uint32_t row, rank, cl, begin, quads, run;  // rank, cl: of the cluster; first token and groups of four tokens of the slice; groups of a thread (odd: no bank conflicts)
+  float xmax, c32, none, reach;          // c32: log2(e) / temp; none: log2 distance from which weights are less than half a unit; reach: or below min_p
+  double xmax_d, c128;                   // 128 log2(e) / temp
+  uint64_t least;                        // what a weight has to have to be drawn: min_p in their units, 1
+  float cut_x;                           // the last token of the run that is kept so far
+  uint32_t cut_idx, tid, warp, lane;
 
   __device__ __forceinline__ uint32_t peer(const void *p, uint32_t cta) const { return cluster_map_shared(p, cta); }
 
   __device__ __forceinline__ float distance(float x) const { return (xmax - x) * c32; }  // in powers of two; never falls where x falls
-  __device__ __forceinline__ uint64_t weight(float x) const {
-    if (x == xmax) return 1ull << a.frac;
-    const double t = ((double)x - (double)xmax) * c64;
-    if (!(t > -64.0 * (a.frac + 1))) return 0u;
-    const double m = t + 6755399441055744.0, f = t - (m - 6755399441055744.0);  // the nearest integer, in the low bits of m; the rest
-    const int k = __double2loint(m);
-    constexpr double L = 0.010830424696249145;  // ln 2 / 64
-    double p = fma(f, L * L * L * L * L / 120.0, L * L * L * L / 24.0);
-    p = fma(f, p, L * L * L / 6.0), p = fma(f, p, L * L / 2.0), p = fma(f, p, L), p = fma(f, p, 1.0);
-    p *= s.pow2[k & 63];
-    p = __hiloint2double(__double2hiint(p) + ((k >> 6) << 20), __double2loint(p));  // at least 2^-2: no underflow
-    return (uint64_t)__double_as_longlong(p + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;  // rounded to an integer
+  // bin of 1/48 of a power of two (a NaN, from an infinity times a zero c32, goes to the last one)
+  __device__ __forceinline__ uint32_t bin_of(float x) const {
+    const float d = distance(x) * 48.0f;
+    return __float_as_uint((d < (float)(SM_BINS - 1) ? d : (float)(SM_BINS - 1)) + 8388608.0f) & 0xFFFFu;
   }
+  __device__ __forceinline__ uint64_t weight(float x) const { return distance(x) <= none ? sm_weight((double)x - xmax_d, c128) : 0u; }
+  __device__ __forceinline__ void weights(const float (&x)[4], uint64_t (&w)[4]) const {
+    double diff[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) diff[e] = (double)x[e] - xmax_d;
+    sm_weights(diff, c128, w);
+#pragma unroll
+    for (int e = 0; e < 4; e++) w[e] = distance(x[e]) <= none ? w[e] : 0u;
+  }
+  __device__ __forceinline__ bool kept(float x, uint32_t i) const { return x > cut_x || (x == cut_x && i <= cut_idx); }
 
-  // f(x, index) for every token of the slice, a thread's in rising order
+  // f(four logits, index of the first) for the tokens of this thread, in rising order
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
-    for (uint32_t q = tid; q * 4u < count; q += SM_THREADS) {
+    const uint32_t q1 = min((tid + 1u) * run, quads);
+#pragma unroll 1
+    for (uint32_t q = tid * run; q < q1; q++) {
       const float4 v = *reinterpret_cast<const float4 *>(xs + 4u * q);
-      f(v.x, begin + 4u * q), f(v.y, begin + 4u * q + 1u), f(v.z, begin + 4u * q + 2u), f(v.w, begin + 4u * q + 3u);
+      const float x[4] = {v.x, v.y, v.z, v.w};
+      f(x, begin + 4u * q);
     }
   }
+  // use(logit, index, weight) for this thread's tokens, in rising order
+  template <typename C>
+  __device__ __forceinline__ void weigh_all(C use) const {
+    each([&](const float (&x)[4], uint32_t i) {
+      uint64_t w[4];
+      weights(x, w);
+#pragma unroll
+      for (uint32_t e = 0; e < 4; e++) use(x[e], i + e, w[e]);
+    });
+    __syncwarp();
+  }
+  // (Whole warps call it.) The same for those that pred(logit, index) picks: 32 looked at at a time, so that few of them cost few
+  // exponentials, not one for every four tokens of which some lane wants one; where a lane has many, all 32 are weighed, four together.
+  template <typename P, typename C>
+  __device__ __forceinline__ void weigh(P pred, C use) const {
+    const uint32_t q1 = min((tid + 1u) * run, quads);
+#pragma unroll 1
+    for (uint32_t g = 0; g < run; g += 8u) {  // (as often in every lane: they meet at its end)
+      const uint32_t qa = tid * run + g, n = qa < q1 ? min(min(8u, run - g), q1 - qa) : 0u;
+      uint32_t mask = 0u;
+#pragma unroll 1
+      for (uint32_t j = 0; j < n; j++) {
+        const float4 v = *reinterpret_cast<const float4 *>(xs + 4u * (qa + j));
+        const uint32_t i = begin + 4u * (qa + j);
+        mask |= ((pred(v.x, i) ? 1u : 0u) | (pred(v.y, i + 1u) ? 2u : 0u) | (pred(v.z, i + 2u) ? 4u : 0u) | (pred(v.w, i + 3u) ? 8u : 0u)) << (4u * j);
+      }
+      if (__any_sync(0xFFFFFFFFu, __popc(mask) > 6)) {
+#pragma unroll 1
+        for (uint32_t j = 0; j < n; j++) {
+          const float4 v = *reinterpret_cast<const float4 *>(xs + 4u * (qa + j));
+          const float x[4] = {v.x, v.y, v.z, v.w};
+          uint64_t w[4];
+          weights(x, w);
+#pragma unroll
+          for (uint32_t e = 0; e < 4; e++)
+            if (mask >> (4u * j + e) & 1u) use(x[e], begin + 4u * (qa + j) + e, w[e]);
+        }
+      } else {
+#pragma unroll 1
+        while (mask) {
+          const uint32_t l = __ffs(mask) - 1u;
+          mask &= mask - 1u;
+          const float x = xs[4u * qa + l];
+          use(x, begin + 4u * qa + l, weight(x));
+        }
+      }
+      __syncwarp();  // (lanes that a branch has parted would go on apart: the dense pass behind a sparse one took three times as long)
+    }
+  }
+  __device__ __forceinline__ uint64_t block_before(uint64_t v, uint64_t &all) const {
+    const ulonglong2 r = sm_before(v, tid);
+    all = r.y;
+    return r.x;
+  }
 
-  // The border of a run in the cluster's histogram: the first bin at which `above` and the bins up to it reach `goal`
-  // (goal_of(mass of all bins)). In: this CTA's hist, complete after a __syncthreads. Out, in every CTA: s.bin and s.above, the mass
-  // ahead of the bin.
-  template <typename G>
-  __device__ void border(uint64_t above, G goal_of) {
-    cluster_sync_all();
-    const uint32_t per_cta = SM_BINS / cl, per = per_cta > SM_THREADS ? per_cta / SM_THREADS : 1u, b0 = rank * per_cta + tid * per;
-    uint64_t v[SM_BINS / SM_THREADS], sum = 0u;
-    for (uint32_t i = 0; i < SM_BINS / SM_THREADS; i++) {
-      v[i] = 0u;
-      if (i < per && tid * per + i < per_cta)
-        for (uint32_t c = 0; c < cl; c++) v[i] += dsm_ld64(peer(&s.hist[b0 + i], c));
-      sum += v[i];
-    }
-    const uint64_t incl = warp_scan64(sum, lane);
-    if (lane == 31) s.wsum[warp] = incl;
+  __device__ __forceinline__ void count(uint32_t bin, uint64_t v) {
+    const uint32_t lo = (uint32_t)v;
+    uint32_t hi = (uint32_t)(v >> 32);
+    if (lo) hi += atomicAdd(&s.low[bin], lo) > ~lo;  // (a carry)
+    if (hi) atomicAdd(&s.high[bin], hi);
+  }
+  __device__ __forceinline__ void clear(uint32_t last) {
+    for (uint32_t i = tid; i < SM_BINS; i += SM_THREADS) s.low[i] = s.high[i] = 0u;
+    if (tid == 0) s.n_mine = 0u, s.n_list = 0u, s.bin = last, s.above = 0u;
     __syncthreads();
-    uint64_t before = incl - sum, mine = 0u;
-    for (uint32_t w = 0; w < SM_WARPS; w++) {
-      if (w < warp) before += s.wsum[w];
-      mine += s.wsum[w];
-    }
-    if (tid < cl) dsm_st64(peer(&s.range[rank], tid), mine);
-    cluster_sync_all();
-    uint64_t all = 0u, ahead = above;
-    for (uint32_t c = 0; c < cl; c++) {
-      if (c < rank) ahead += s.range[c];
-      all += s.range[c];
-    }
+  }
+  // The bin of v (three to a thread) at which the bins up to it reach goal_of(sum of all): s.bin, and s.above the mass ahead of it.
+  template <typename G>
+  __device__ __forceinline__ void bin_at(const uint64_t (&v)[SM_PER], G goal_of) {
+    uint64_t all, before = block_before(v[0] + v[1] + v[2], all);
     const uint64_t goal = goal_of(all);
-    before += ahead;
-    for (uint32_t i = 0; i < SM_BINS / SM_THREADS; i++) {
-      if (before < goal && goal <= before + v[i])  // one thread of the cluster
-        for (uint32_t c = 0; c < cl; c++) dsm_st32(peer(&s.bin, c), b0 + i), dsm_st64(peer(&s.above, c), before);
+#pragma unroll
+    for (uint32_t i = 0; i < SM_PER; i++) {
+      if (before < goal && goal <= before + v[i]) s.bin = SM_PER * tid + i, s.above = before;  // one thread
       before += v[i];
     }
+    __syncthreads();
+  }
+  // The same of the cluster's histogram, in every CTA.
+  template <typename G>
+  __device__ __forceinline__ void border(G goal_of) {
     cluster_sync_all();
+    for (uint32_t b = rank * (SM_BINS / cl) + tid; b < (rank + 1u) * (SM_BINS / cl); b += SM_THREADS) {  // this CTA's share of the bins, for all
+      uint32_t lo[SM_MAX_CL], hi[SM_MAX_CL];
+#pragma unroll
+      for (uint32_t c = 0; c < SM_MAX_CL; c++) lo[c] = c < cl ? dsm_ld32(peer(&s.low[b], c)) : 0u, hi[c] = c < cl ? dsm_ld32(peer(&s.high[b], c)) : 0u;
+      uint64_t v = 0u;
+#pragma unroll
+      for (uint32_t c = 0; c < SM_MAX_CL; c++) v += (uint64_t)hi[c] << 32 | lo[c];
+      for (uint32_t c = 0; c < cl; c++) dsm_st64(peer(&s.bins[b], c), v);
+    }
+    cluster_sync_all();
+    const uint64_t v[SM_PER] = {s.bins[SM_PER * tid], s.bins[SM_PER * tid + 1u], s.bins[SM_PER * tid + 2u]};
+    bin_at(v, goal_of);
   }
 
-  // The tokens that `in` picks into the first CTA's list; how many there are (more than SM_LIST: the list is not whole).
-  template <typename F>
-  __device__ uint32_t gather(F in) {
-    if (tid == 0) s.n_mine = 0u, s.n_list = 0u;
-    cluster_sync_all();
-    each([&](float x, uint32_t i) {
-      if (in(x, i)) {
-        const uint32_t at = atomicAdd(&s.n_mine, 1u);
-        if (at < SM_LIST) s.mine[at] = (uint64_t)sm_key(x) << 32 | (uint32_t)~i;
-      }
-    });
+  // A candidate, into this CTA's list.
+  __device__ __forceinline__ void add(float x, uint32_t i) {
+    const uint32_t at = atomicAdd(&s.n_mine, 1u);
+    if (at < SM_LIST) s.mine[at] = (uint64_t)sm_key(x) << 32 | (uint32_t)~i;
+  }
+  // The CTAs' lists into the first CTA's; how many there are (more than SM_LIST: it is not whole). s.n_mine and s.n_list are zeroed a cluster
+  // barrier ahead of the first add().
+  __device__ __forceinline__ uint32_t gather() {
     __syncthreads();
     const uint32_t n = s.n_mine;
     if (tid < cl && n) {  // every CTA counts them all (nobody looks into another CTA's memory behind the last barrier: it may have ended)
@@ -183,18 +306,31 @@ struct Sampler {
     return s.n_list;
   }
 
-  // v[0 .. n - 1] falling (one CTA; n at most SM_LIST, room up to the next power of two; the fill sorts to the end)
-  __device__ void sort_falling(uint64_t *v, uint32_t n) const {
+  // s.list[0 .. n - 1] falling into s.mine (one CTA; n at most SM_LIST).
+  __device__ void sort_falling(uint32_t n) {
+    if (n <= (uint32_t)SM_SHORT) {  // by counting, for each, those ahead of it, two threads each (100 .. 256 values: 500 .. 1800 cycles, below 2000 .. 4500)
+      const uint32_t half = (n + 1u) / 2u, i = tid >> 1, j0 = tid & 1u ? half : 0u, j1 = tid & 1u ? n : half;
+      const uint64_t v = i < n ? s.list[i] : 0u;
+      uint32_t before = 0u;
+      if (i < n) {
+#pragma unroll 8
+        for (uint32_t j = j0; j < j1; j++) before += s.list[j] > v;
+      }
+      before += __shfl_xor_sync(0xFFFFFFFFu, before, 1);
+      if (i < n && !(tid & 1u)) s.mine[before] = v;
+      __syncthreads();
+      return;
+    }
     uint32_t m = 2u;
     while (m < n) m <<= 1;
-    for (uint32_t i = n + tid; i < m; i += SM_THREADS) v[i] = 0u;
+    for (uint32_t i = tid; i < m; i += SM_THREADS) s.mine[i] = i < n ? s.list[i] : 0u;  // (the fill sorts to the end)
     __syncthreads();
     for (uint32_t size = 2; size <= m; size <<= 1)
       for (uint32_t step = size >> 1; step; step >>= 1) {
         for (uint32_t t = tid; t < m / 2u; t += SM_THREADS) {
           const uint32_t i = 2u * t - (t & (step - 1u)), j = i + step;
-          const uint64_t p = v[i], q = v[j];
-          if ((p < q) == ((i & size) == 0u)) v[i] = q, v[j] = p;
+          const uint64_t p = s.mine[i], q = s.mine[j];
+          if ((p < q) == ((i & size) == 0u)) s.mine[i] = q, s.mine[j] = p;
         }
         // pairs up to 32 apart stay within the 64 values of a warp, this step and the next ones
         if (step > 32u || (step == 1u && size >= 64u)) __syncthreads();
@@ -203,327 +339,324 @@ struct Sampler {
     __syncthreads();
   }
 
-  // The sum of f over the CTA's threads ahead of this one, and of all of them.
-  __device__ uint64_t block_before(uint64_t v, uint64_t &all) {
-    const uint64_t incl = warp_scan64(v, lane);
-    __syncthreads();
-    if (lane == 31) s.wsum[warp] = incl;
-    __syncthreads();
-    uint64_t before = incl - v;
-    all = 0u;
-    for (uint32_t w = 0; w < SM_WARPS; w++) {
-      if (w < warp) before += s.wsum[w];
-      all += s.wsum[w];
+  // The rest of the row in the first CTA alone: of its n candidates, which are the row's first ones, the first k (at most one per thread), of
+  // these the run that reaches goal_of(mass of the k), of these the ones of `least`, and the draw.
+  template <typename G>
+  __device__ __forceinline__ void finish(uint32_t n, uint32_t k, float u, G goal_of) {
+    sort_falling(n);
+    uint64_t all, v = tid < k ? weight(sm_unkey((uint32_t)(s.mine[tid] >> 32))) : 0u;
+    const uint64_t before = block_before(v, all);
+    const bool keep = tid < k && before < goal_of(all) && v >= least;
+    if (keep) s.w[tid] = v;
+    const uint32_t m = (uint32_t)__syncthreads_count(keep);  // a run from the top
+    // by index: the sum of the kept ones ahead of each, four threads to one of them
+#pragma unroll 1
+    for (uint32_t i0 = 0; i0 < m; i0 += SM_THREADS / 4u) {
+      const uint32_t i = i0 + tid / 4u;
+      uint64_t ahead = 0u, sum = 0u;
+      const uint32_t me = i < m ? ~(uint32_t)s.mine[i] : 0u;
+      if (i < m) {
+#pragma unroll 4
+        for (uint32_t j = tid & 3u; j < m; j += 4u) {
+          const uint64_t w = s.w[j];
+          sum += w;
+          if (~(uint32_t)s.mine[j] < me) ahead += w;
+        }
+      }
+      ahead += __shfl_xor_sync(0xFFFFFFFFu, ahead, 1), sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
+      ahead += __shfl_xor_sync(0xFFFFFFFFu, ahead, 2), sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
+      if (i < m && (tid & 3u) == 0u) {
+        const uint64_t goal = sample_goal(u, sum), w = s.w[i];
+        if (ahead <= goal && goal < ahead + w) sample_out(a, row, me, (float)((double)w / (double)sum));  // one thread
+      }
     }
-    return before;
-  }
-
-  __device__ __forceinline__ bool kept(float x, uint32_t i) const {
-    const uint32_t k = sm_key(x);
-    return k > s.cut_key || (k == s.cut_key && i <= s.cut_idx);
   }
 
   // The cut (the last kept token of the run) at which the mass of the kept tokens, taken from the top, reaches a goal. MASS: weights, the
-  // goal p times the mass of all kept; otherwise counts, the goal k.
+  // goal p times the mass of all kept; otherwise counts, the goal k. True: the first CTA has done the rest of the row (MASS, u).
   template <bool MASS>
-  __device__ void cut_run(double p, uint32_t k) {
-    auto mass = [&](float x) { return MASS ? weight(x) : (uint64_t)1u; };
-    uint64_t goal = k;
-    auto goal_of = [&](uint64_t all) {
-      const double g = ceil(p * (double)all);
-      return g < 1.0 ? (uint64_t)1u : min(all, (uint64_t)g);
-    };
-    // round 0: bins of the weights (MASS); then 11, 11 and 10 bits of the key
+  __device__ __forceinline__ bool cut_run(float p, uint32_t k, float u) {
+    uint64_t goal = k, above = 0u;
+    // round 0: bins of the weights; then 10, 10, 10 and 2 bits of the key
     uint32_t coarse = 0u, prefix = 0u, bits = 0u;  // the bin of round 0, the leading bits of the key so far
-    auto in_prefix = [&](float x) {
-      return (!MASS || min((uint32_t)(SM_BINS - 1), (uint32_t)(distance(x) * 64.0f)) == coarse) && (bits == 0u || sm_key(x) >> (32u - bits) == prefix);
-    };
-    uint64_t above = 0u;
-    for (int round = MASS ? 0 : 1; round < 4; round++) {
-      const uint32_t w = round == 3 ? 10u : 11u;
-      for (uint32_t i = tid; i < SM_BINS; i += SM_THREADS) s.hist[i] = 0u;
-      __syncthreads();
+#pragma unroll 1
+    for (int round = 0; round < 5; round++) {
+      const uint32_t w = round == 0 ? 0u : round == 4 ? 2u : 10u, last = round == 0 ? SM_BINS - 1u : (1u << w) - 1u;
+      auto member = [&](float x, uint32_t i) {
+        return kept(x, i) && (round == 0 || (bin_of(x) == coarse && (bits == 0u || sm_key(x) >> (32u - bits) == prefix)));
+      };
+      auto bin = [&](float x) { return round == 0 ? bin_of(x) : last - ((sm_key(x) >> (32u - bits - w)) & last); };
+      clear(last);
+      if (!MASS)
+        each([&](const float (&x)[4], uint32_t i) {
+#pragma unroll
+          for (uint32_t e = 0; e < 4; e++)
+            if (member(x[e], i + e)) count(bin(x[e]), 1u);
+        });
+      else if (round == 0 && cut_idx == SM_NONE) weigh_all([&](float x, uint32_t, uint64_t v) { count(bin_of(x), v); });
+      else weigh(member, [&](float x, uint32_t, uint64_t v) { count(bin(x), v); });
+      border([&](uint64_t all) {
+        if (MASS && round == 0) goal = run_goal(p, all);
+        return goal - above;
+      });
+      const uint32_t b = s.bin;
+      const uint64_t ahead = s.above;
       if (MASS && round == 0) {
-        each([&](float x, uint32_t i) {
-          if (kept(x, i)) {
-            const uint64_t v = weight(x);
-            if (v) atomicAdd(reinterpret_cast<unsigned long long *>(&s.hist[min((uint32_t)(SM_BINS - 1), (uint32_t)(distance(x) * 64.0f))]), (unsigned long long)v);
+        // A run of few tokens goes to the first CTA whole. How many are in the bins up to b: their masses over their weights, 1 % off.
+        float about = 0.0f;
+#pragma unroll
+        for (uint32_t i = 0; i < SM_PER; i++)
+          if (SM_PER * tid + i <= b) about += (float)s.bins[SM_PER * tid + i] * exp2f((float)(SM_PER * tid + i) * (1.0f / 48.0f) - (float)a.frac);
+        about = warp_sum_all(about);
+        if (lane == 0) s.max_of[warp] = about;  // (no longer needed for what it is)
+        __syncthreads();
+        about = 0.0f;
+        for (int i = 0; i < SM_WARPS; i++) about += s.max_of[i];
+        if (about <= 400.0f) {
+          each([&](const float (&x)[4], uint32_t i) {
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++)
+              if (bin_of(x[e]) <= b && kept(x[e], i + e)) add(x[e], i + e);
+          });
+          const uint32_t n = gather();
+          if (n <= (uint32_t)SM_THREADS) {
+            if (rank == 0u) finish(n, n, u, [&](uint64_t) { return goal; });
+            return true;
           }
-        });
-        border(0u, [&](uint64_t all) { return goal = goal_of(all); });
-        coarse = s.bin;
-      } else {
-        each([&](float x, uint32_t i) {
-          if (kept(x, i) && in_prefix(x)) {
-            const uint32_t digit = (sm_key(x) >> (32u - bits - w)) & ((1u << w) - 1u);
-            atomicAdd(reinterpret_cast<unsigned long long *>(&s.hist[(1u << w) - 1u - digit]), (unsigned long long)mass(x));
-          }
-        });
-        border(above, [&](uint64_t) { return goal; });
-        prefix = prefix << w | ((1u << w) - 1u - s.bin), bits += w;
+          __syncthreads();  // (everybody has read the count)
+          if (tid == 0) s.n_mine = 0u, s.n_list = 0u;
+          cluster_sync_all();
+        }
       }
-      above = s.above;
-      const uint32_t n = gather([&](float x, uint32_t i) { return kept(x, i) && in_prefix(x); });
+      __syncthreads();  // (everybody has read the bins: the lists lie there)
+      each([&](const float (&x)[4], uint32_t i) {
+#pragma unroll
+        for (uint32_t e = 0; e < 4; e++)
+          if (bin(x[e]) == b && member(x[e], i + e)) add(x[e], i + e);
+      });
+      const uint32_t n = gather();
+      above += ahead;
+      if (round == 0) coarse = b;
+      else prefix = prefix << w | (last - b), bits += w;
       if (n <= (uint32_t)SM_LIST) {
         if (rank == 0u) {
-          sort_falling(s.list, n);
+          sort_falling(n);
           uint64_t at = above;
+#pragma unroll 1
           for (uint32_t i0 = 0; i0 < n; i0 += SM_THREADS) {  // at most two rounds
             uint64_t all;
             const uint32_t i = i0 + tid;
-            const uint64_t v = i < n ? mass(sm_unkey((uint32_t)(s.list[i] >> 32))) : 0u, before = at + block_before(v, all);
+            const uint64_t e = i < n ? s.mine[i] : 0u;
+            const uint64_t v = i < n ? (MASS ? weight(sm_unkey((uint32_t)(e >> 32))) : 1u) : 0u, before = at + block_before(v, all);
             if (i < n && before < goal && goal <= before + v)  // one thread
-              for (uint32_t c = 0; c < cl; c++) dsm_st32(peer(&s.cut_key, c), (uint32_t)(s.list[i] >> 32)), dsm_st32(peer(&s.cut_idx, c), ~(uint32_t)s.list[i]);
+              for (uint32_t c = 0; c < cl; c++) dsm_st64(peer(&s.cut, c), e);
             at += all;
           }
         }
         cluster_sync_all();
-        return;
+        cut_x = sm_unkey((uint32_t)(s.cut >> 32)), cut_idx = ~(uint32_t)s.cut;
+        return false;
       }
+      __syncthreads();  // (everybody has read the count)
     }
     // what is left are equal logits: as many of them as the goal takes, by index
     const float x = sm_unkey(prefix);
-    const uint64_t w = mass(x), need = (goal - above + w - 1u) / w;
-    uint32_t idx;
-    uint64_t v, all;
-    locate([&](float y, uint32_t i) { return (uint64_t)(kept(y, i) && sm_key(y) == prefix); }, [&](uint64_t) { return need - 1u; }, idx, v, all);
-    cluster_sync_all();  // (everybody has read the old cut)
-    if (tid == 0) s.cut_key = prefix, s.cut_idx = idx;
-    __syncthreads();
+    const uint64_t w = MASS ? weight(x) : 1u, need = (goal - above + w - 1u) / w;
+    locate<false>([&](float y, uint32_t i) { return kept(y, i) && y == x; }, [&](uint64_t) { return need - 1u; },
+                  [&](uint32_t idx, uint64_t, uint64_t) {
+                    for (uint32_t c = 0; c < cl; c++) dsm_st32(peer(&s.base, c), idx);
+                  });
+    cluster_sync_all();
+    cut_x = x, cut_idx = s.base;
+    return false;
   }
 
-  // The first token, by index, at which the running sum of f exceeds goal_of(sum of all); its f and the sum. In every CTA (idx is SM_NONE if
-  // there is none).
-  template <typename F, typename G>
-  __device__ void locate(F f, G goal_of, uint32_t &idx, uint64_t &value, uint64_t &all) {
-    // sums of the 128 tokens that a warp takes at a time, in the order of the indices: [step][warp]
-    uint64_t *part = s.hist;
-    const uint32_t quads = (count + 3u) / 4u, steps = (quads + SM_THREADS - 1u) / SM_THREADS;
-    __syncthreads();
-    if (tid == 0) s.bin = SM_NONE;
-    uint64_t mine = 0u;
-    auto quad = [&](uint32_t q, uint64_t (&v)[4]) {
-      v[0] = v[1] = v[2] = v[3] = 0u;
-      if (q < quads) {
-        const float4 x = *reinterpret_cast<const float4 *>(xs + 4u * q);
-        v[0] = f(x.x, begin + 4u * q), v[1] = f(x.y, begin + 4u * q + 1u), v[2] = f(x.z, begin + 4u * q + 2u), v[3] = f(x.w, begin + 4u * q + 3u);
-      }
-    };
-    for (uint32_t k = 0; k < steps; k++) {
-      uint64_t v[4];
-      quad(k * SM_THREADS + tid, v);
-      const uint64_t sum = warp_sum64(v[0] + v[1] + v[2] + v[3]);
-      if (lane == 0) part[k * SM_WARPS + warp] = sum;
-      mine += sum;
+  // The first token, by index, at which the running sum over those that pred(logit, index) picks exceeds goal_of(sum of all): found(index, its
+  // part, the sum) in one thread of the cluster (in none if there is no such token). MASS: the sum of their weights of `least` and more,
+  // otherwise their number.
+  template <bool MASS, typename P, typename G, typename H>
+  __device__ __forceinline__ void locate(P pred, G goal_of, H found) {
+    uint64_t sum = 0u, mine, all = 0u;
+    if (MASS && cut_idx == SM_NONE && reach == none) {  // everything is in
+      weigh_all([&](float, uint32_t, uint64_t w) { sum += w; });
+    } else if (MASS) {
+      weigh(pred, [&](float, uint32_t, uint64_t w) { sum += w >= least ? w : 0u; });
+    } else {
+      each([&](const float (&x)[4], uint32_t i) {
+#pragma unroll
+        for (uint32_t e = 0; e < 4; e++) sum += pred(x[e], i + e);
+      });
     }
-    if (lane == 0) s.wsum[warp] = mine;
-    __syncthreads();
-    mine = 0u;
-    for (uint32_t w = 0; w < SM_WARPS; w++) mine += s.wsum[w];
-    if (tid < cl) dsm_st64(peer(&s.range[rank], tid), mine);
+    uint64_t before = block_before(sum, mine);
+    if (tid < cl) dsm_st64(peer(&s.part[rank], tid), mine);
     cluster_sync_all();
-    uint64_t before = 0u;
-    all = 0u;
     for (uint32_t c = 0; c < cl; c++) {
-      if (c < rank) before += s.range[c];
-      all += s.range[c];
+      if (c < rank) before += s.part[c];
+      all += s.part[c];
     }
     const uint64_t goal = goal_of(all);
-    if (warp == 0 && before <= goal && goal < before + mine) {  // one CTA: the step and warp, then the token
-      uint32_t at = 0u;
-      for (uint32_t p0 = 0; p0 < steps * SM_WARPS; p0 += 32u) {
-        const uint64_t v = p0 + lane < steps * SM_WARPS ? part[p0 + lane] : 0u, incl = before + warp_scan64(v, lane);
-        const uint32_t over = __ballot_sync(0xFFFFFFFFu, incl > goal);
-        if (over) {
-          const int l = __ffs(over) - 1;
-          at = p0 + l, before = __shfl_sync(0xFFFFFFFFu, incl - v, l);
-          break;
+    const uint32_t at = __ballot_sync(0xFFFFFFFFu, before <= goal && goal < before + sum);  // one thread of the cluster; its warp takes its run
+    if (!at) return;
+    const int owner = __ffs(at) - 1;
+    uint64_t base = __shfl_sync(0xFFFFFFFFu, before, owner);
+    const uint32_t q0 = (warp * 32u + owner) * run, q1 = min(q0 + run, quads);
+#pragma unroll 1
+    for (uint32_t qa = q0; qa < q1; qa += 32u) {
+      const uint32_t q = qa + lane;
+      uint64_t v[4] = {0u, 0u, 0u, 0u};
+      if (q < q1) {
+        const float4 y = *reinterpret_cast<const float4 *>(xs + 4u * q);
+        const float x[4] = {y.x, y.y, y.z, y.w};
+        if (MASS) weights(x, v);
+#pragma unroll
+        for (uint32_t e = 0; e < 4; e++) {
+          const bool in = pred(x[e], begin + 4u * q + e);
+          v[e] = MASS ? (in && v[e] >= least ? v[e] : 0u) : in;
         }
-        before = __shfl_sync(0xFFFFFFFFu, incl, 31);
       }
-      const uint32_t q = (at / SM_WARPS) * SM_THREADS + (at % SM_WARPS) * 32u + lane;
-      uint64_t v[4];
-      quad(q, v);
-      uint64_t run = before + warp_scan64(v[0] + v[1] + v[2] + v[3], lane) - (v[0] + v[1] + v[2] + v[3]);
+      const uint64_t four = (v[0] + v[1]) + (v[2] + v[3]), incl = warp_scan64(four, lane);
+      uint64_t at_sum = base + incl - four;
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        if (run <= goal && goal < run + v[e])  // one thread of the cluster
-          for (uint32_t c = 0; c < cl; c++) dsm_st32(peer(&s.bin, c), begin + 4u * q + e), dsm_st64(peer(&s.above, c), v[e]);
-        run += v[e];
+        if (at_sum <= goal && goal < at_sum + v[e]) found(begin + 4u * q + e, v[e], all);
+        at_sum += v[e];
       }
+      base += __shfl_sync(0xFFFFFFFFu, incl, 31);
     }
-    cluster_sync_all();
-    idx = s.bin, value = s.above;
   }
 };
 
-// u times the sum as a running sum of integers is compared with: exceeded means at least one more
-__device__ __forceinline__ uint64_t sample_goal(float u, uint64_t all) {
-  const double g = (double)u * (double)all;
-  return g > 0.0 ? min((uint64_t)min(g, 9.2e18), all - 1u) : 0u;
-}
-
-__device__ __forceinline__ void sample_out(const SampleArgs &a, uint32_t row, uint32_t idx, float prob) {
-  uint32_t *o = reinterpret_cast<uint32_t *>(reinterpret_cast<char *>(a.out) + a.out_stride * row);
-  o[0] = idx, o[1] = __float_as_uint(prob);
-}
-
-__global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleArgs a) {
-  extern __shared__ __align__(16) uint8_t smem_s[];
-  SampleSmem &s = *reinterpret_cast<SampleSmem *>(smem_s);
+__global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(const SampleArgs a) {
+  SampleSmem &s = sm_front();
+  float *xs = reinterpret_cast<float *>(smem_s + SM_FRONT);
   cluster_arrive();  // (waited for ahead of the first store into a peer, which has to run by then)
   pdl_prologue();
   const uint32_t row = blockIdx.x / a.cl, rank = blockIdx.x % a.cl, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cl = a.cl;
-  const uint32_t begin = min(a.n, rank * a.slice), count = min(a.n, begin + a.slice) - begin;
-  float *xs = reinterpret_cast<float *>(smem_s + ((sizeof(SampleSmem) + 15u) & ~(size_t)15u));
-  const float temp = a.temp ? a.temp[row] : 1.0f, top_p = a.top_p ? a.top_p[row] : 1.0f, min_p = a.min_p ? a.min_p[row] : 0.0f, u = a.u[row];
-  const uint32_t top_k = a.top_k ? a.top_k[row] : 0u;
-  const bool greedy = !(temp > 0.0f), by_k = !greedy && top_k > 0u && top_k < a.n;
+  const uint32_t begin = min(a.n, rank * a.slice), count = min(a.n, begin + a.slice) - begin, quads = (count + 3u) / 4u;
 
-  // ---- the slice, its maximum, and the threads' own maxima
-  for (uint32_t i = tid; i < SM_BINS / 2u; i += SM_THREADS) s.hist[i] = 0u;  // 2048 counts of 32 bits
+  // ---- the slice; meanwhile the settings
   const float *x = reinterpret_cast<const float *>(reinterpret_cast<const char *>(a.x) + a.x_stride * row) + begin;
-  float mx = -INFINITY;
-  uint32_t mi = SM_NONE;
-  for (uint32_t q = tid; q * 4u < count; q += SM_THREADS) {
-    float v[4];
+  for (uint32_t q = tid; q < quads; q += SM_THREADS) {
     if (a.wide && q * 4u + 4u <= count) {
-      const float4 f = *reinterpret_cast<const float4 *>(x + 4u * q);
-      v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+      __pipeline_memcpy_async(xs + 4u * q, x + 4u * q, 16);
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; e++) v[e] = q * 4u + e < count ? x[4u * q + e] : -INFINITY;
+      for (uint32_t e = 0; e < 4; e++) {
+        if (q * 4u + e < count) __pipeline_memcpy_async(xs + 4u * q + e, x + 4u * q + e, 4);
+        else xs[4u * q + e] = -INFINITY;
+      }
     }
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      if (!(v[e] >= -INFINITY)) v[e] = -INFINITY;  // a NaN is never drawn
-      if (v[e] > mx) mx = v[e], mi = begin + 4u * q + e;
-    }
-    *reinterpret_cast<float4 *>(xs + 4u * q) = make_float4(v[0], v[1], v[2], v[3]);
   }
+  __pipeline_commit();
+  const float temp = a.temp ? a.temp[row] : 1.0f, top_p = a.top_p ? a.top_p[row] : 1.0f, min_p = a.min_p ? a.min_p[row] : 0.0f, u = a.u[row];
+  const uint32_t top_k = a.top_k ? a.top_k[row] : 0u;
+  const bool greedy = !(temp > 0.0f), by_k = !greedy && top_k > 0u && top_k < a.n, by_p = top_p < 1.0f;  // (a NaN: off)
+  const double c128 = greedy ? 0.0 : 184.6649652337873 / (double)temp;  // 128 log2(e) / temp
+  const float mp = min_p > 0.0f ? fminf(min_p, 1.0f) : 0.0f, none = (float)(a.frac + 1);
+  Sampler S = {a, s, xs, row, rank, cl, begin, quads, ((quads + SM_THREADS - 1u) / SM_THREADS) | 1u, 0.0f, (float)fmin(c128 / 128.0, 3.4e38), none,
+               fminf(none, mp > 0.0f ? 0.01f - log2f(mp) : none), 0.0, c128, max((uint64_t)1u, (uint64_t)ceil((double)mp * (double)(1ull << a.frac))), -INFINITY,
+               SM_NONE, tid, warp, lane};
+  if (tid < SM_TABLE && !greedy) s.pow2[tid] = scalbn(exp2((double)tid / SM_TABLE), a.frac);
+  if (tid == 0) s.n_mine = 0u, s.n_list = 0u;
+  __pipeline_wait_prior(0);
   __syncthreads();
-  uint32_t *counts = reinterpret_cast<uint32_t *>(s.hist);
-  if (by_k) atomicAdd(&counts[SM_BINS - 1u - (sm_key(mx) >> 21)], 1u);
-  {
-    float bv = mx;
-    uint32_t bi = mi;
-    for (int o = 16; o; o >>= 1) {
-      const float ov = __shfl_xor_sync(0xFFFFFFFFu, bv, o);
-      const uint32_t oi = __shfl_xor_sync(0xFFFFFFFFu, bi, o);
-      if (ov > bv || (ov == bv && oi < bi)) bv = ov, bi = oi;
-    }
-    if (lane == 0) s.wsum[warp] = (uint64_t)sm_key(bv) << 32 | (uint32_t)~bi;
-  }
-  if (tid < 64u) s.pow2[tid] = scalbn(exp2((double)tid / 64.0), a.frac);
-  __syncthreads();
-  cluster_wait();
-  if (warp == 0) {
-    uint64_t b = lane < SM_WARPS ? s.wsum[lane] : 0u;
-    for (int o = 16; o; o >>= 1) b = max(b, (uint64_t)__shfl_xor_sync(0xFFFFFFFFu, b, o));
-    if (lane < cl) {
-      dsm_st32(cluster_map_shared(&s.max_v[rank], lane), __float_as_uint(sm_unkey((uint32_t)(b >> 32))));
-      dsm_st32(cluster_map_shared(&s.max_i[rank], lane), ~(uint32_t)b);
-    }
-  }
-  if (by_k) {  // the bin of the threads' maxima at which j of them are reached, its lower end
-    const uint32_t j = (top_k + cl - 1u) / cl;
-    uint32_t c4[4], sum = 0u;
+
+  // ---- maxima: of groups of cl threads, 512 of them in the row, for everybody (greedy: of the CTAs, with the first index of each)
+  float mx = -INFINITY;
+  S.each([&](const float (&v)[4], uint32_t i) {
+    if (v[0] != v[0] || v[1] != v[1] || v[2] != v[2] || v[3] != v[3]) {  // a NaN is never drawn
 #pragma unroll
-    for (int e = 0; e < 4; e++) c4[e] = counts[4u * tid + e], sum += c4[e];
-    uint32_t incl = sum;
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
-      if ((int)lane >= o) incl += v;
+      for (int e = 0; e < 4; e++)
+        if (v[e] != v[e]) xs[i - begin + e] = -INFINITY;
     }
-    uint32_t *ws = reinterpret_cast<uint32_t *>(s.wsum + SM_WARPS);
-    if (lane == 31) ws[warp] = incl;
-    if (tid == 0) s.bin = SM_NONE;
-    __syncthreads();
-    uint32_t before = incl - sum;
-    for (uint32_t w = 0; w < warp; w++) before += ws[w];
+    mx = fmaxf(fmaxf(mx, fmaxf(v[0], v[1])), fmaxf(v[2], v[3]));  // (fmaxf passes over a NaN)
+  });
+  __syncwarp();
+  if (greedy) {
+    uint32_t at = SM_NONE;
+    const float wm = warp_max(mx);
+    if (mx == wm && wm > -INFINITY)
+      S.each([&](const float (&v)[4], uint32_t i) {
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-      if (before < j && j <= before + c4[e]) s.bin = 4u * tid + e;
-      before += c4[e];
-    }
+        for (int e = 3; e >= 0; e--)
+          if (v[e] == wm) at = min(at, i + e);
+      });
+    __syncwarp();
+    at = __reduce_min_sync(0xFFFFFFFFu, at);
+    if (lane == 0) s.wsum[warp] = (uint64_t)sm_key(wm) << 32 | (uint32_t)~at;
     __syncthreads();
-    if (tid < cl) dsm_st32(cluster_map_shared(&s.floor_key[rank], tid), s.bin == SM_NONE ? 0u : (SM_BINS - 1u - s.bin) << 21);
-  }
-  cluster_sync_all();
-  float xmax = -INFINITY;
-  uint32_t imax = SM_NONE, floor_key = SM_NONE;
-  for (uint32_t c = 0; c < cl; c++) {
-    if (s.max_v[c] > xmax) xmax = s.max_v[c], imax = s.max_i[c];
-    if (by_k) floor_key = min(floor_key, s.floor_key[c]);
-  }
-  if (greedy || imax == SM_NONE) {
-    if (rank == 0u && tid == 0u) sample_out(a, row, imax, imax == SM_NONE ? 0.0f : 1.0f);
+    cluster_wait();
+    if (tid == 0) {
+      uint64_t b = 0u;
+      for (int w = 0; w < SM_WARPS; w++) b = max(b, s.wsum[w]);
+      dsm_st32(S.peer(&s.first[rank], 0u), ~(uint32_t)b), dsm_st32(S.peer(&s.max_of[rank], 0u), __float_as_uint(sm_unkey((uint32_t)(b >> 32))));
+    }
+    cluster_sync_all();
+    if (rank == 0u && tid == 0u) {
+      uint32_t first = SM_NONE;
+      float best = -INFINITY;
+      for (uint32_t c = 0; c < cl; c++)
+        if (s.max_of[c] > best) best = s.max_of[c], first = s.first[c];
+      sample_out(a, row, first, first == SM_NONE ? 0.0f : 1.0f);
+    }
     return;
   }
+  float own = mx;
+  for (uint32_t o = 1; o < cl; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
+  cluster_wait();
+  dsm_st32(S.peer(&s.max_of[rank * (SM_THREADS / cl) + tid / cl], tid % cl), __float_as_uint(mx));  // (a thread of each group for each CTA)
+  cluster_sync_all();
+  mx = s.max_of[tid];
+  const float wm = warp_max(mx);
+  if (lane == 0) s.wsum[warp] = __float_as_uint(wm);
+  __syncthreads();
+  float xmax = warp_max(lane < SM_WARPS ? __uint_as_float((uint32_t)s.wsum[lane]) : -INFINITY);
+  if (xmax == -INFINITY) {
+    if (rank == 0u && tid == 0u) sample_out(a, row, SM_NONE, 0.0f);
+    return;
+  }
+  if (xmax == INFINITY) {  // its tokens, equally likely, and no other
+    S.each([&](const float (&v)[4], uint32_t i) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) xs[i - begin + e] = v[e] == INFINITY ? 0.0f : -INFINITY;
+    });
+    xmax = 0.0f, mx = mx == INFINITY ? 0.0f : -INFINITY, own = own == INFINITY ? 0.0f : -INFINITY;
+    __syncthreads();
+  }
+  S.xmax = xmax, S.xmax_d = xmax;
 
-  Sampler S = {a, s, xs, rank, cl, begin, count, xmax, 0.0f, 0.0, 0.0, 0.0f, tid, warp, lane};
-  S.c64 = 64.0 * 1.4426950408889634 / (double)temp, S.c32 = (float)(S.c64 / 64.0);
-  const float mp = min_p > 0.0f ? fminf(min_p, 1.0f) : 0.0f;
-  S.min_w = (double)mp * (double)(1ull << a.frac);
-  S.far = fminf((float)(a.frac + 2), mp > 0.0f ? 0.01f - log2f(mp) : INFINITY);
-  const bool by_p = top_p < 1.0f;  // (a NaN: off)
-  auto heavy = [&](uint64_t w) { return w && (double)w >= S.min_w; };
-
-  if (by_k && top_k <= (uint32_t)SM_LIST) {
-    const uint32_t n = S.gather([&](float v, uint32_t) { return sm_key(v) >= floor_key && v > -INFINITY; });
+  if (by_k && top_k <= (uint32_t)SM_THREADS) {
+    // a lower bound of the k-th largest of the 512 maxima, bit by bit from the top, until less than a quarter more of them reach it
+    const uint32_t key = sm_key(mx);
+    uint32_t low = 0u;
+#pragma unroll 1
+    for (uint32_t bit = 1u << 31; bit >= 1u << 8; bit >>= 1) {
+      const uint32_t reached = (uint32_t)__syncthreads_count(key >= (low | bit));
+      if (reached >= top_k) {
+        low |= bit;
+        if (reached <= top_k + top_k / 4u) break;
+      }
+    }
+    const float floor_x = sm_unkey(max(low, 0x00800000u));  // (the lowest finite float: -inf is none)
+    if (own >= floor_x)
+      S.each([&](const float (&v)[4], uint32_t i) {
+        if (fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])) >= floor_x) {
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            if (v[e] >= floor_x) S.add(v[e], i + e);
+        }
+      });
+    const uint32_t n = S.gather();
     if (n <= (uint32_t)SM_LIST) {
-      if (rank != 0u) return;
-      S.sort_falling(s.list, n);
-      const uint32_t k = min(top_k, n);
-      uint64_t w[2], before[2], sums[2] = {0u, 0u};
-#pragma unroll
-      for (int r = 0; r < 2; r++) {
-        const uint32_t i = r * SM_THREADS + tid;
-        w[r] = i < k ? S.weight(sm_unkey((uint32_t)(s.list[i] >> 32))) : 0u;
-        before[r] = S.block_before(w[r], sums[r]);
-      }
-      before[1] += sums[0];
-      const double g = by_p ? (double)top_p * (double)(sums[0] + sums[1]) : INFINITY;
-#pragma unroll
-      for (int r = 0; r < 2; r++) {  // what is kept, by index: (~index, place)
-        const uint32_t i = r * SM_THREADS + tid;
-        const bool keep = i < k && ((double)before[r] < g || i == 0u) && heavy(w[r]);
-        if (i < k) s.mine[i] = keep ? (s.list[i] << 32 | i) : 0u;
-        if (i < k) s.hist[i] = w[r];
-      }
-      __syncthreads();
-      S.sort_falling(s.mine, k);  // (tokens left out go to the end; index 0xFFFFFFFF does not exist, so no kept one is 0)
-#pragma unroll
-      for (int r = 0; r < 2; r++) {
-        const uint32_t i = r * SM_THREADS + tid;
-        const uint64_t e = i < k ? s.mine[i] : 0u;
-        w[r] = e ? s.hist[(uint32_t)e] : 0u;
-        before[r] = S.block_before(w[r], sums[r]);
-      }
-      before[1] += sums[0];
-      const uint64_t all = sums[0] + sums[1], goal = sample_goal(u, all);
-#pragma unroll
-      for (int r = 0; r < 2; r++)
-        if (before[r] <= goal && goal < before[r] + w[r])  // one thread
-          sample_out(a, row, ~(uint32_t)(s.mine[r * SM_THREADS + tid] >> 32), (float)((double)w[r] / (double)all));
+      if (rank == 0u) S.finish(n, min(top_k, n), u, [&](uint64_t all) { return by_p ? run_goal(top_p, all) : all; });
       return;
     }
+    __syncthreads();  // (everybody has read the count)
   }
-  if (tid == 0) s.cut_key = 0u, s.cut_idx = SM_NONE;
-  __syncthreads();
-  if (by_k) S.cut_run<false>(0.0, top_k);
-  if (by_p) S.cut_run<true>((double)top_p, 0u);
-  uint32_t idx;
-  uint64_t w, all;
-  S.locate(
-      [&](float v, uint32_t i) {
-        if (!(S.distance(v) <= S.far) && v != xmax) return (uint64_t)0u;
-        if (!S.kept(v, i)) return (uint64_t)0u;
-        const uint64_t r = S.weight(v);
-        return heavy(r) ? r : (uint64_t)0u;
-      },
-      [&](uint64_t sum) { return sample_goal(u, sum); }, idx, w, all);
-  if (rank == 0u && tid == 0u) sample_out(a, row, idx, (float)((double)w / (double)all));
+  if (by_k) S.cut_run<false>(0.0f, top_k, u);
+  if (by_p && S.cut_run<true>(top_p, 0u, u)) return;
+  S.locate<true>([&](float v, uint32_t i) { return S.distance(v) <= S.reach && S.kept(v, i); }, [&](uint64_t sum) { return sample_goal(u, sum); },
+                 [&](uint32_t idx, uint64_t w, uint64_t all) { sample_out(a, row, idx, (float)((double)w / (double)all)); });
 }
 
 // CTAs of a row
@@ -548,7 +681,7 @@ extern "C" int ie_b200_sample(const float *d_x, uint32_t n, uint32_t *d_out, con
   int log2n = 0;
   while ((1u << log2n) < n) log2n++;
   a.frac = 62 - log2n < 50 ? 62 - log2n : 50;
-  const size_t smem = ((sizeof(SampleSmem) + 15u) & ~(size_t)15u) + (size_t)a.slice * 4u;
+  const size_t smem = SM_FRONT + (size_t)a.slice * 4u;
   if (int r = ensure_dynamic_smem(reinterpret_cast<const void *>(sample_kernel), smem)) return r;
   const cudaError_t e = launch_pdl_cluster(sample_kernel, dim3(T * a.cl), dim3(SM_THREADS), smem, static_cast<cudaStream_t>(stream), a.cl, a);
   count_launch();
