@@ -202,7 +202,8 @@ struct Sampler {
     __syncwarp();
   }
   // (Whole warps call it.) The same for those that pred(logit, index) picks: 32 looked at at a time, so that few of them cost few
-  // exponentials, not one for every four tokens of which some lane wants one; where a lane has many, all 32 are weighed, four together.
+  // exponentials, not one for every four tokens of which some lane wants one; where a lane has many, all 32 are weighed, four together, and
+  // the others used with a weight of 0.
   template <typename P, typename C>
   __device__ __forceinline__ void weigh(P pred, C use) const {
     const uint32_t q1 = min((tid + 1u) * run, quads);
@@ -225,7 +226,7 @@ struct Sampler {
           weights(x, w);
 #pragma unroll
           for (uint32_t e = 0; e < 4; e++)
-            if (mask >> (4u * j + e) & 1u) use(x[e], begin + 4u * (qa + j) + e, w[e]);
+            use(x[e], begin + 4u * (qa + j) + e, mask >> (4u * j + e) & 1u ? w[e] : 0u);
         }
       } else {
 #pragma unroll 1
@@ -440,15 +441,41 @@ struct Sampler {
       else prefix = prefix << w | (last - b), bits += w;
       if (n <= (uint32_t)SM_LIST) {
         if (rank == 0u) {
-          sort_falling(n);
           uint64_t at = above;
+          uint32_t m = n;
+          if (m > (uint32_t)SM_SHORT) {  // a histogram of the list first (a sort of 1024 takes 8000 cycles)
+            auto fine = [&](float x) {
+              if (round == 0) return min((uint32_t)(SM_BINS - 1), (uint32_t)fmaxf((distance(x) * 48.0f - ((float)b - 0.5f)) * (float)SM_BINS, 0.0f));
+              return 1023u - ((sm_key(x) << bits) >> 22);
+            };
+            auto mass = [&](float x) { return MASS ? weight(x) : 1u; };
+            __syncthreads();
+            clear(SM_BINS - 1u);
+            for (uint32_t i = tid; i < m; i += SM_THREADS) {
+              const float x = sm_unkey((uint32_t)(s.list[i] >> 32));
+              count(fine(x), mass(x));
+            }
+            __syncthreads();
+            uint64_t v[SM_PER];
+#pragma unroll
+            for (uint32_t i = 0; i < SM_PER; i++) v[i] = (uint64_t)s.high[SM_PER * tid + i] << 32 | s.low[SM_PER * tid + i];
+            bin_at(v, [&](uint64_t) { return goal - above; });
+            at += s.above;
+            for (uint32_t i = tid; i < m; i += SM_THREADS)
+              if (fine(sm_unkey((uint32_t)(s.list[i] >> 32))) == s.bin) s.mine[atomicAdd(&s.n_mine, 1u)] = s.list[i];
+            __syncthreads();
+            m = s.n_mine;
+            for (uint32_t i = tid; i < m; i += SM_THREADS) s.list[i] = s.mine[i];
+            __syncthreads();
+          }
+          sort_falling(m);
 #pragma unroll 1
-          for (uint32_t i0 = 0; i0 < n; i0 += SM_THREADS) {  // at most two rounds
+          for (uint32_t i0 = 0; i0 < m; i0 += SM_THREADS) {  // at most two rounds
             uint64_t all;
             const uint32_t i = i0 + tid;
-            const uint64_t e = i < n ? s.mine[i] : 0u;
-            const uint64_t v = i < n ? (MASS ? weight(sm_unkey((uint32_t)(e >> 32))) : 1u) : 0u, before = at + block_before(v, all);
-            if (i < n && before < goal && goal <= before + v)  // one thread
+            const uint64_t e = i < m ? s.mine[i] : 0u;
+            const uint64_t v = i < m ? (MASS ? weight(sm_unkey((uint32_t)(e >> 32))) : 1u) : 0u, before = at + block_before(v, all);
+            if (i < m && before < goal && goal <= before + v)  // one thread
               for (uint32_t c = 0; c < cl; c++) dsm_st64(peer(&s.cut, c), e);
             at += all;
           }
