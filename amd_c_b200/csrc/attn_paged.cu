@@ -25,7 +25,7 @@
 
 namespace ieb {
 
-constexpr int AP_WARPS = 4, AP_THREADS = 32 * AP_WARPS, AP_STAGES = 3, AP_HEADS = 8;
+constexpr int AP_HEADS = 8;
 constexpr uint32_t AP_MAX_CTAS = 1024u;  // the counters at the front of the scratch
 
 struct PagedAttnArgs {
@@ -41,17 +41,21 @@ struct PagedAttnArgs {
   float scale_log2;  // log2(e) / sqrt(hd)
 };
 
-template <typename KV, int HD>
+// W: warps of a CTA
+template <typename KV, int HD, int W>
 struct ApGeom {
   static constexpr bool F16 = sizeof(KV) == 2;
+  static constexpr int THREADS = 32 * W, STAGES = HD == 32 ? 5 : HD == 128 ? 3 : W == 4 ? 4 : F16 ? 3 : 5;  // buffers of a warp
   static constexpr int CH = F16 ? 16 : 8;                       // positions of a chunk
   static constexpr int ROWB = HD * (int)sizeof(KV), PIECES = ROWB / 16, PER_LANE = CH * PIECES / 32;
   static constexpr int STAGE = 2 * CH * ROWB;                   // K rows, then V rows
-  static constexpr int RED_ROW = HD + 4;                        // floats between the heads of a record (banks: 4 per head pair)
-  static constexpr int RING_OFF = 0, RED_OFF = AP_WARPS * AP_STAGES * STAGE, ML_OFF = RED_OFF + AP_WARPS * AP_HEADS * RED_ROW * 4,
-                       VALID_OFF = ML_OFF + AP_WARPS * AP_HEADS * 8, MISC_OFF = VALID_OFF + AP_WARPS * AP_STAGES * 4, TOTAL = MISC_OFF + 64,
+  static constexpr int REC_ROW = HD + 4;                        // floats between the heads of a record in global memory: outputs, max, sum
+  static constexpr int RING_OFF = 0, RED_OFF = W * STAGES * STAGE, ML_OFF = RED_OFF + W * AP_HEADS * HD * 4,
+                       VALID_OFF = ML_OFF + W * AP_HEADS * 8, MISC_OFF = (VALID_OFF + W * STAGES * 4 + 15) / 16 * 16, TOTAL = MISC_OFF + 128,
                        Q_OFF = RED_OFF;  // float cache: the unit's q, until its records are written
-  static constexpr int FIT = 228 * 1024 / (TOTAL + 1024), CTAS = FIT < 4 ? FIT : 4;  // CTAs that an SM's shared memory holds
+  static constexpr int FIT = 228 * 1024 / (TOTAL + 1024), MOST = F16 || W == 4 ? 16 / W : 1, CTAS = FIT < MOST ? FIT : MOST;  // on an SM: what its shared memory and 128 registers a thread allow
+  // Output d of head h in a warp's record in shared memory: the four head pairs that a store of the MMA's layout meets lie in different banks.
+  __device__ static __forceinline__ uint32_t red_at(uint32_t h, uint32_t d) { return h * HD + (d ^ (h >> 1 & 3u) * 8u); }
   // The 16-byte pieces of a row change places so that the reads of eight rows (ldmatrix), or of two rows by four lanes each, meet
   // eight different bank groups.
   __device__ static __forceinline__ uint32_t at(uint32_t row, uint32_t piece) {
@@ -83,27 +87,29 @@ __device__ __forceinline__ void ap_split2(float x, float y, uint32_t &hi, uint32
 }
 
 // ---- a warp's part of the arithmetic: its running maximum (log2 units), sum and outputs of the unit's heads
-template <typename KV, int HD>
+template <typename KV, int HD, int W>
 struct ApWarp;
 
-template <int HD>
-struct ApWarp<__half, HD> {
-  using Gm = ApGeom<__half, HD>;
+template <int HD, int W>
+struct ApWarp<__half, HD, W> {
+  using Gm = ApGeom<__half, HD, W>;
   static constexpr int KS = HD / 16;
+  float2 q[KS][2];                // the next unit's q, on its way
   uint32_t qh[KS][2], ql[KS][2];  // B fragments of Q^T[16 dims x heads]: column lane / 4
   float o[KS][4], m[2], l[2];     // o[u][j], o[u][2 + j]: head 2 (lane % 4) + j, dims 16 u + lane / 4, + 8
 
-  __device__ __forceinline__ void start(const float *q, uint32_t heads, const uint8_t *, int lane) {
-    const uint32_t h = lane >> 2, tq = lane & 3;
+  __device__ __forceinline__ void load(const float *src, uint32_t heads, uint32_t tid) {
+    const uint32_t h = (tid & 31u) >> 2, tq = tid & 3u;
+#pragma unroll
+    for (int k = 0; k < KS; k++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) q[k][e] = h < heads ? *reinterpret_cast<const float2 *>(src + h * HD + 16 * k + 2 * tq + 8 * e) : make_float2(0.f, 0.f);
+  }
+  __device__ __forceinline__ void start(uint32_t, float *, uint32_t) {
 #pragma unroll
     for (int k = 0; k < KS; k++) {
-      float2 a = make_float2(0.f, 0.f), b = a;
-      if (h < heads) {
-        a = *reinterpret_cast<const float2 *>(q + h * HD + 16 * k + 2 * tq);
-        b = *reinterpret_cast<const float2 *>(q + h * HD + 16 * k + 2 * tq + 8);
-      }
-      ap_split2(a.x, a.y, qh[k][0], ql[k][0]);
-      ap_split2(b.x, b.y, qh[k][1], ql[k][1]);
+#pragma unroll
+      for (int e = 0; e < 2; e++) ap_split2(q[k][e].x, q[k][e].y, qh[k][e], ql[k][e]);
 #pragma unroll
       for (int e = 0; e < 4; e++) o[k][e] = 0.0f;
     }
@@ -155,7 +161,7 @@ struct ApWarp<__half, HD> {
       for (int e = 0; e < 4; e++) o[u][e] = fmaf(o[u][e], al[e & 1], c[e]);
     }
   }
-  // this warp's record: red [heads][RED_ROW] outputs (2^15 times), ml [heads][2]
+  // this warp's record: red [heads][HD] outputs (2^15 times; red_at), ml [heads][2]
   __device__ __forceinline__ void finish(float *red, float *ml, int lane) {
     const uint32_t hq = lane >> 2, tq = lane & 3;
 #pragma unroll
@@ -166,21 +172,32 @@ struct ApWarp<__half, HD> {
       sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 16);
       const uint32_t h = 2 * tq + j;
 #pragma unroll
-      for (int u = 0; u < KS; u++) red[h * Gm::RED_ROW + 16 * u + hq] = o[u][j], red[h * Gm::RED_ROW + 16 * u + hq + 8] = o[u][2 + j];
+      for (int u = 0; u < KS; u++) red[Gm::red_at(h, 16 * u + hq)] = o[u][j], red[Gm::red_at(h, 16 * u + hq + 8)] = o[u][2 + j];
       if (hq == 0) ml[2 * h] = m[j], ml[2 * h + 1] = sum * 0x1p15f;
     }
   }
 };
 
-template <int HD>
-struct ApWarp<float, HD> {
-  using Gm = ApGeom<float, HD>;
+template <int HD, int W>
+struct ApWarp<float, HD, W> {
+  using Gm = ApGeom<float, HD, 4>;
   static constexpr int DPL = HD / 32;  // output dims of a lane
   float o[AP_HEADS][DPL], m[AP_HEADS], l[AP_HEADS];
+  static constexpr int QPT = AP_HEADS * HD / (32 * W);
+  float q[QPT];  // this thread's part of the next unit's q, on its way
   const float *qs;
+  bool few;
 
-  __device__ __forceinline__ void start(const float *, uint32_t, const uint8_t *q_smem, int) {
-    qs = reinterpret_cast<const float *>(q_smem);
+  __device__ __forceinline__ void load(const float *src, uint32_t heads, uint32_t tid) {
+#pragma unroll
+    for (int i = 0; i < QPT; i++) q[i] = tid + 32u * W * i < heads * HD ? src[tid + 32u * W * i] : 0.0f;
+  }
+  // (All threads call it, behind a barrier after which nobody reads what is at q_smem.)
+  __device__ __forceinline__ void start(uint32_t heads, float *q_smem, uint32_t tid) {
+    few = heads <= 4u, qs = q_smem;
+#pragma unroll
+    for (int i = 0; i < QPT; i++) q_smem[tid + 32u * W * i] = q[i];
+    __syncthreads();
 #pragma unroll
     for (int h = 0; h < AP_HEADS; h++) {
       m[h] = -INFINITY, l[h] = 0.0f;
@@ -188,23 +205,25 @@ struct ApWarp<float, HD> {
       for (int d = 0; d < DPL; d++) o[h][d] = 0.0f;
     }
   }
-  __device__ __forceinline__ void chunk(uint8_t *stage, uint32_t valid, float scale_log2, int lane) {
+  // H: heads worked on, 4 or 8 (half the arithmetic where the unit has no more than four)
+  template <int H>
+  __device__ __forceinline__ void chunk_of(uint8_t *stage, uint32_t valid, float scale_log2, int lane) {
     const uint32_t pos = lane >> 2, part = lane & 3;  // lane: a quarter of the dims of one position
-    float s[AP_HEADS], al[AP_HEADS];
+    float s[H], al[H];
 #pragma unroll
-    for (int h = 0; h < AP_HEADS; h++) s[h] = 0.0f;
+    for (int h = 0; h < H; h++) s[h] = 0.0f;
 #pragma unroll 4
     for (int i = 0; i < HD / 16; i++) {
       const uint32_t piece = 4 * i + part;
       const float4 k = *reinterpret_cast<const float4 *>(stage + Gm::at(pos, piece));
 #pragma unroll
-      for (int h = 0; h < AP_HEADS; h++) {
+      for (int h = 0; h < H; h++) {
         const float4 x = *reinterpret_cast<const float4 *>(qs + h * HD + 4 * piece);
         s[h] = fmaf(x.x, k.x, s[h]), s[h] = fmaf(x.y, k.y, s[h]), s[h] = fmaf(x.z, k.z, s[h]), s[h] = fmaf(x.w, k.w, s[h]);
       }
     }
 #pragma unroll
-    for (int h = 0; h < AP_HEADS; h++) {
+    for (int h = 0; h < H; h++) {
       s[h] += __shfl_xor_sync(0xFFFFFFFFu, s[h], 1);
       s[h] += __shfl_xor_sync(0xFFFFFFFFu, s[h], 2);
       if (pos >= valid) s[h] = -INFINITY;
@@ -222,17 +241,17 @@ struct ApWarp<float, HD> {
     __syncwarp();
     if (part == 0) {
 #pragma unroll
-      for (int h = 0; h < AP_HEADS; h += 4) *reinterpret_cast<float4 *>(stage + pos * 32u + 4 * h) = make_float4(s[h], s[h + 1], s[h + 2], s[h + 3]);
+      for (int h = 0; h < H; h += 4) *reinterpret_cast<float4 *>(stage + pos * 32u + 4 * h) = make_float4(s[h], s[h + 1], s[h + 2], s[h + 3]);
     }
     __syncwarp();
 #pragma unroll
-    for (int h = 0; h < AP_HEADS; h++)
+    for (int h = 0; h < H; h++)
 #pragma unroll
       for (int d = 0; d < DPL; d++) o[h][d] *= al[h];
     const uint8_t *vs = stage + Gm::CH * Gm::ROWB;
 #pragma unroll
     for (int j = 0; j < Gm::CH; j++) {
-      float v[DPL], w[AP_HEADS];
+      float v[DPL], w[H];
       const uint8_t *at = vs + Gm::at(j, (lane * DPL) / 4) + ((lane * DPL) & 3) * 4;
       if (DPL == 4) {
         const float4 x = *reinterpret_cast<const float4 *>(at);
@@ -244,15 +263,19 @@ struct ApWarp<float, HD> {
         v[0] = *reinterpret_cast<const float *>(at);
       }
 #pragma unroll
-      for (int h = 0; h < AP_HEADS; h += 4) {
+      for (int h = 0; h < H; h += 4) {
         const float4 x = *reinterpret_cast<const float4 *>(stage + j * 32u + 4 * h);
         w[h] = x.x, w[h + 1] = x.y, w[h + 2] = x.z, w[h + 3] = x.w;
       }
 #pragma unroll
-      for (int h = 0; h < AP_HEADS; h++)
+      for (int h = 0; h < H; h++)
 #pragma unroll
         for (int d = 0; d < DPL; d++) o[h][d] = fmaf(w[h], v[d], o[h][d]);
     }
+  }
+  __device__ __forceinline__ void chunk(uint8_t *stage, uint32_t valid, float scale_log2, int lane) {
+    if (few) chunk_of<4>(stage, valid, scale_log2, lane);
+    else chunk_of<8>(stage, valid, scale_log2, lane);
   }
   __device__ __forceinline__ void finish(float *red, float *ml, int lane) {
 #pragma unroll
@@ -262,7 +285,7 @@ struct ApWarp<float, HD> {
       sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 8);
       sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 16);
 #pragma unroll
-      for (int d = 0; d < DPL; d++) red[h * Gm::RED_ROW + lane * DPL + d] = o[h][d];
+      for (int d = 0; d < DPL; d++) red[Gm::red_at(h, lane * DPL + d)] = o[h][d];
       if (lane == 0) ml[2 * h] = m[h], ml[2 * h + 1] = sum;
     }
   }
@@ -271,7 +294,7 @@ struct ApWarp<float, HD> {
 // Where a CTA's share stands: chunks [j, j1) of unit `unit` of row r (this share's part of it), and what is left behind them.
 struct ApCursor {
   uint32_t r, seq, len, unit, j0, j1;
-  uint64_t left;
+  uint64_t left, first;  // chunk numbers left behind j1; number of the unit's first chunk
 };
 
 // Positions and sequence of row r: 0 positions where the row pads the batch.
@@ -280,82 +303,115 @@ __device__ __forceinline__ uint32_t ap_row(const PagedAttnArgs &a, uint32_t r, u
   return seq < a.kv.n_seq ? min(__ldg(a.len + r), table_positions(a.kv)) : 0u;
 }
 
-template <typename KV, int HD>
-__global__ void __launch_bounds__(AP_THREADS, ApGeom<KV, HD>::CTAS) attn_paged_kernel(const PagedAttnArgs a) {
-  using Gm = ApGeom<KV, HD>;
+template <typename KV, int HD, int W>
+__global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_kernel(const PagedAttnArgs a) {
+  using Gm = ApGeom<KV, HD, W>;
+  constexpr int WARPS = W, THREADS = 32 * W, STAGES = Gm::STAGES;
   constexpr uint32_t CH = Gm::CH;
   extern __shared__ __align__(128) uint8_t smem_ap[];
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  uint8_t *ring = smem_ap + Gm::RING_OFF + warp * AP_STAGES * Gm::STAGE;
+  uint8_t *ring = smem_ap + Gm::RING_OFF + warp * STAGES * Gm::STAGE;
   float *red = reinterpret_cast<float *>(smem_ap + Gm::RED_OFF), *ml = reinterpret_cast<float *>(smem_ap + Gm::ML_OFF);
-  uint32_t *valid_of = reinterpret_cast<uint32_t *>(smem_ap + Gm::VALID_OFF) + warp * AP_STAGES, *misc = reinterpret_cast<uint32_t *>(smem_ap + Gm::MISC_OFF);
+  uint32_t *valid_of = reinterpret_cast<uint32_t *>(smem_ap + Gm::VALID_OFF) + warp * STAGES, *misc = reinterpret_cast<uint32_t *>(smem_ap + Gm::MISC_OFF);
   uint64_t *misc64 = reinterpret_cast<uint64_t *>(misc);
   pdl_prologue();
   const uint32_t units = a.kv.n_kv * a.groups;
 
-  // ---- the share: chunks [x0, x1) of all, and the row it starts in
-  uint32_t per = (a.R + AP_THREADS - 1u) / AP_THREADS, r_lo = min(a.R, tid * per), r_hi = min(a.R, r_lo + per);
-  uint64_t mine = 0u;
-  for (uint32_t r = r_lo; r < r_hi; r++) {
+  // ---- the share: chunks [x0, x1) of all, and the row it starts in. Where there are few units, each is numbered as if it had whole
+  // shares, if that makes them little longer: a CTA then has a part of one unit only.
+  const uint32_t per = (a.R + THREADS - 1u) / THREADS, r_lo = min(a.R, tid * per), r_hi = min(a.R, r_lo + per);
+  auto chunks = [&](uint32_t r) {
     uint32_t seq;
-    mine += (ap_row(a, r, seq) + CH - 1u) / CH;
+    return (ap_row(a, r, seq) + CH - 1u) / CH;
+  };
+  auto block_sum = [&](uint64_t mine, uint64_t &before) {  // of all threads, and of those ahead
+    uint64_t incl = mine, all = 0u;
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint64_t v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+      if ((int)lane >= o) incl += v;
+    }
+    __syncthreads();
+    if (lane == 31) misc64[warp] = incl;
+    __syncthreads();
+    before = incl - mine;
+    for (uint32_t w = 0; w < WARPS; w++) {
+      const uint64_t v = misc64[w];
+      if (w < warp) before += v;
+      all += v;
+    }
+    return all;
+  };
+  // Behind the chunks of a unit come some numbers without any, for what its end costs (about as long as a chunk of each warp).
+  constexpr uint32_t END = WARPS;
+  uint64_t before, mine = 0u;
+  for (uint32_t r = r_lo; r < r_hi; r++) {
+    const uint32_t lc = chunks(r);
+    mine += lc ? lc + END : 0u;
   }
-  uint64_t incl = mine;
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint64_t v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
-    if ((int)lane >= o) incl += v;
-  }
-  if (lane == 31) misc64[warp] = incl;
-  __syncthreads();
-  uint64_t before = incl - mine, all = 0u;
-  for (uint32_t w = 0; w < AP_WARPS; w++) {
-    const uint64_t v = misc64[w];
-    if (w < warp) before += v;
-    all += v;
-  }
-  all *= units, before *= units, mine *= units;
-  uint64_t share = (all + gridDim.x - 1u) / gridDim.x;
+  uint64_t all = block_sum(mine, before) * units, share = (all + gridDim.x - 1u) / gridDim.x;
   if (share < a.min_share) share = a.min_share;
+  uint32_t whole_shares = 1u;  // more: unit lengths are rounded up to a multiple of this
+  if ((uint64_t)a.R * units <= gridDim.x) {
+    for (uint32_t more = 0; more <= 3u * WARPS / 2u; more += WARPS / 4u) {
+      const uint32_t s = (uint32_t)share + more;
+      uint64_t parts = 0u, ahead;
+      for (uint32_t r = r_lo; r < r_hi; r++) parts += (chunks(r) + s - 1u) / s;
+      const uint64_t all_parts = block_sum(parts, ahead) * units;
+      if (all_parts <= gridDim.x) {
+        share = whole_shares = s, all = all_parts * s, before = ahead * s, mine = parts * s;
+        break;
+      }
+    }
+  }
+  before *= units, mine *= units;
+  auto numbered = [&](uint32_t lc) { return whole_shares > 1u ? (lc + whole_shares - 1u) / whole_shares * whole_shares : lc ? lc + END : 0u; };  // of a unit of lc chunks
   const uint64_t x0 = min(all, share * blockIdx.x), x1 = min(all, x0 + share);
   if (x0 < x1 && before <= x0 && x0 < before + mine) {  // one thread
-    uint32_t r = r_lo, seq;
+    uint32_t r = r_lo;
     uint64_t row;
     for (;; r++) {
-      row = (uint64_t)((ap_row(a, r, seq) + CH - 1u) / CH) * units;
+      row = (uint64_t)numbered(chunks(r)) * units;
       if (x0 < before + row) break;
       before += row;
     }
-    misc[8] = r, misc64[5] = x0 - before;  // row, chunk of the row
+    misc[16] = r, misc64[9] = x0 - before;  // row, chunk of the row
   }
   __syncthreads();
 
   if (x0 < x1) {
     ApCursor c;  // what is worked on
     {
-      c.r = misc[8];
+      c.r = misc[16];
       c.len = ap_row(a, c.r, c.seq);
-      const uint32_t lc = (c.len + CH - 1u) / CH;
-      const uint64_t at = misc64[5];
-      c.unit = (uint32_t)(at / lc), c.j0 = (uint32_t)(at - (uint64_t)c.unit * lc);
-      c.left = x1 - x0;
-      c.j1 = (uint32_t)min((uint64_t)lc, c.j0 + c.left);
-      c.left -= c.j1 - c.j0;
+      const uint32_t lc = (c.len + CH - 1u) / CH, num = numbered(lc);
+      const uint64_t at = misc64[9];
+      c.unit = (uint32_t)(at / num), c.j0 = (uint32_t)(at - (uint64_t)c.unit * num);
+      c.first = x0 - c.j0;
+      const uint64_t end = min(c.first + num, x1);  // of the share's numbers in this unit
+      c.left = x1 - end, c.j1 = (uint32_t)min((uint64_t)lc, end - c.first);
     }
     auto advance = [&](ApCursor &k) {  // to the next unit (k.left > 0: there is one)
+      k.first = x1 - k.left;
       if (++k.unit == units) {
         k.unit = 0u;
         do k.len = ap_row(a, ++k.r, k.seq);
         while (k.len == 0u);
       }
-      k.j0 = 0u, k.j1 = (uint32_t)min((uint64_t)((k.len + CH - 1u) / CH), k.left);
-      k.left -= k.j1;
+      const uint32_t lc = (k.len + CH - 1u) / CH;
+      const uint64_t end = min(k.first + numbered(lc), x1);
+      k.left = x1 - end, k.j0 = 0u, k.j1 = (uint32_t)min((uint64_t)lc, end - k.first);
     };
+    bool any = true;
+    if (c.j0 >= c.j1) {  // the share starts behind the chunks of a unit
+      any = c.left != 0u;
+      if (any) advance(c);
+    }
 
-    // ---- the ring: this warp's chunks, in the order in which they are worked on, AP_STAGES - 1 ahead
+    // ---- the ring: this warp's chunks, in the order in which they are worked on, STAGES - 1 ahead
     ApCursor f = c;  // what is fetched
     uint32_t fj = f.j0 + warp, f_num = 0u, f_stage = 0u;
     const uint32_t cpp = a.kv.page / CH;
-    bool more = true;
+    bool more = any;
     auto find = [&] {  // the next chunk of this warp and its page number (needed only one chunk later: nobody waits for it)
       while (fj >= f.j1) {
         if (f.left == 0u) {
@@ -384,54 +440,62 @@ __global__ void __launch_bounds__(AP_THREADS, ApGeom<KV, HD>::CTAS) attn_paged_k
           __pipeline_memcpy_async(st + CH * Gm::ROWB + to, vs + src, 16, in ? 0 : 16);
         }
         if (lane == 0) valid_of[f_stage] = valid;
-        fj += AP_WARPS;
+        fj += WARPS;
         find();
       }
       __pipeline_commit();
-      f_stage = f_stage + 1u == AP_STAGES ? 0u : f_stage + 1u;
+      f_stage = f_stage + 1u == STAGES ? 0u : f_stage + 1u;
     };
-    find();
+    if (any) find();
 #pragma unroll
-    for (int i = 0; i < AP_STAGES - 1; i++) fetch();
+    for (int i = 0; i < STAGES - 1; i++) fetch();
 
-    ApWarp<KV, HD> w;
+    ApWarp<KV, HD, W> w;
+    auto heads_of = [&](const ApCursor &k, uint32_t &h0) {  // the first head of the cursor's unit, and how many
+      const uint32_t kvh = k.unit / a.groups, grp = k.unit - kvh * a.groups;
+      h0 = kvh * a.G + grp * a.gw;
+      return min(a.gw, a.G - grp * a.gw);
+    };
+    auto load_q = [&](const ApCursor &k) {
+      uint32_t h0;
+      const uint32_t heads = heads_of(k, h0);
+      w.load(reinterpret_cast<const float *>(reinterpret_cast<const char *>(a.q) + a.q_stride * k.r) + (size_t)h0 * HD, heads, tid);
+    };
+    if (any) load_q(c);
     uint32_t stage = 0u;
-    uint64_t x = x0;  // global number of chunk c.j0 of the unit
-    while (true) {
-      const uint32_t kvh = c.unit / a.groups, grp = c.unit - kvh * a.groups, h0 = kvh * a.G + grp * a.gw, heads = min(a.gw, a.G - grp * a.gw);
-      const float *q = reinterpret_cast<const float *>(reinterpret_cast<const char *>(a.q) + a.q_stride * c.r) + (size_t)h0 * HD;
-      if (!Gm::F16) {
-        float *qs = reinterpret_cast<float *>(smem_ap + Gm::Q_OFF);  // (the barriers at the end of a unit: nobody reads the last one's any more)
-        for (uint32_t i = tid; i < AP_HEADS * HD; i += AP_THREADS) qs[i] = i < heads * HD ? q[i] : 0.0f;
-        __syncthreads();
-      }
-      w.start(q, heads, smem_ap + Gm::Q_OFF, lane);
-      for (uint32_t j = c.j0 + warp; j < c.j1; j += AP_WARPS) {
-        __pipeline_wait_prior(AP_STAGES - 2);
+    while (any) {
+      uint32_t h0;
+      const uint32_t heads = heads_of(c, h0);
+      w.start(heads, reinterpret_cast<float *>(smem_ap + Gm::Q_OFF), tid);
+      for (uint32_t j = c.j0 + warp; j < c.j1; j += WARPS) {
+        __pipeline_wait_prior(STAGES - 2);
         __syncwarp();
         const uint32_t valid = valid_of[stage];
         fetch();
         w.chunk(ring + stage * Gm::STAGE, valid, a.scale_log2, lane);
-        stage = stage + 1u == AP_STAGES ? 0u : stage + 1u;
+        stage = stage + 1u == STAGES ? 0u : stage + 1u;
       }
-      // ---- the warps' records meet
-      if (!Gm::F16) __syncthreads();  // (q lies where they go)
-      w.finish(red + warp * AP_HEADS * Gm::RED_ROW, ml + warp * AP_HEADS * 2, lane);
+      // ---- the warps' records meet; the next unit's q sets out meanwhile
+      ApCursor next = c;
+      const bool go_on = c.left != 0u;
+      if (go_on) advance(next), load_q(next);
+      if (!Gm::F16) __syncthreads();  // (q lies where the records go)
+      w.finish(red + warp * AP_HEADS * HD, ml + warp * AP_HEADS * 2, lane);
       __syncthreads();
       const uint32_t lc = (c.len + CH - 1u) / CH;
       const bool whole = c.j0 == 0u && c.j1 == lc;
-      constexpr uint32_t QUADS = HD / 4, REC = AP_HEADS * Gm::RED_ROW;
-      for (uint32_t i0 = warp * 32u; i0 < heads * QUADS; i0 += AP_THREADS) {
+      constexpr uint32_t QUADS = HD / 4, REC = AP_HEADS * Gm::REC_ROW;
+      for (uint32_t i0 = warp * 32u; i0 < heads * QUADS; i0 += THREADS) {
         const uint32_t i = i0 + lane, h = min(i / QUADS, AP_HEADS - 1u), d = i % QUADS * 4u;
         float M = -INFINITY, L = 0.0f;
 #pragma unroll
-        for (int k = 0; k < AP_WARPS; k++) M = fmaxf(M, ml[k * AP_HEADS * 2 + 2 * h]);
+        for (int k = 0; k < WARPS; k++) M = fmaxf(M, ml[k * AP_HEADS * 2 + 2 * h]);
         const float base = M == -INFINITY ? 0.0f : M;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int k = 0; k < AP_WARPS; k++) {
+        for (int k = 0; k < WARPS; k++) {
           const float f = ex2(ml[k * AP_HEADS * 2 + 2 * h] - base);
-          const float4 v = *reinterpret_cast<const float4 *>(red + k * REC + h * Gm::RED_ROW + d);
+          const float4 v = *reinterpret_cast<const float4 *>(red + k * AP_HEADS * HD + Gm::red_at(h, d));
           L = fmaf(f, ml[k * AP_HEADS * 2 + 2 * h + 1], L);
           acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
         }
@@ -441,7 +505,7 @@ __global__ void __launch_bounds__(AP_THREADS, ApGeom<KV, HD>::CTAS) attn_paged_k
           acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
           store_row4<HD>(a.out, a.out_stride, a.oq, a.oq_stride, a.wide, a.n_head * HD / 32u, c.r, h0 + h, d, acc, in);
         } else if (in) {
-          float *to = a.rec + ((size_t)blockIdx.x * 2u + (c.j0 == 0u ? 1u : 0u)) * REC + h * Gm::RED_ROW;
+          float *to = a.rec + ((size_t)blockIdx.x * 2u + (c.j0 == 0u ? 1u : 0u)) * REC + h * Gm::REC_ROW;
           *reinterpret_cast<float4 *>(to + d) = acc;
           if (d == 0u) to[HD] = M, to[HD + 1] = L;
         }
@@ -449,45 +513,63 @@ __global__ void __launch_bounds__(AP_THREADS, ApGeom<KV, HD>::CTAS) attn_paged_k
       if (!whole) {
         // The parts of the unit, in the order of its positions: the second record of the CTA it starts in, then the first ones of the
         // CTAs behind. Whoever is the last to have written adds them up.
-        const uint64_t u0 = x - c.j0;
+        const uint64_t u0 = c.first;
         const uint32_t c0 = (uint32_t)(u0 / share), parts = (uint32_t)((u0 + lc - 1u) / share) - c0 + 1u;
         __threadfence();
         __syncthreads();
         if (tid == 0) {
           const bool last = atomicAdd(&a.count[c0], 1u) == parts - 1u;
           if (last) a.count[c0] = 0u;  // left zero for the next launch
-          misc[12] = last;
+          misc[20] = last;
         }
         __syncthreads();
-        if (misc[12]) {
+        if (misc[20]) {
           __threadfence();
-          for (uint32_t i0 = warp * 32u; i0 < heads * QUADS; i0 += AP_THREADS) {
-            const uint32_t i = i0 + lane, h = min(i / QUADS, heads - 1u), d = i % QUADS * 4u;
-            const float *rec = a.rec + (size_t)c0 * 2u * REC + h * Gm::RED_ROW;
+          // A warp per head, or per several heads of fewer than 128 dims: the lanes share out the parts' (max, sum) and their weights, then
+          // FLIGHT parts at a time are on their way.
+          constexpr uint32_t PER_WARP = 32u / QUADS, FLIGHT = HD == 128 ? 16u : 8u;  // heads; parts (as the registers allow)
+          for (uint32_t g = warp; g * PER_WARP < heads; g += WARPS) {
+            const uint32_t h = g * PER_WARP + lane / QUADS, hh = min(h, heads - 1u), d = lane % QUADS * 4u;
+            const float *rec = a.rec + (size_t)c0 * 2u * REC + hh * Gm::REC_ROW;
             auto part = [&](uint32_t k) { return rec + (size_t)(2u * k + (k == 0u ? 1u : 0u)) * REC; };
             float M = -INFINITY, L = 0.0f;
-            for (uint32_t k = i % QUADS; k < parts; k += QUADS) M = fmaxf(M, __ldcg(part(k) + HD));
-#pragma unroll
-            for (uint32_t o = 1; o < (QUADS < 32u ? QUADS : 32u); o <<= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, o));
-            const float base = M == -INFINITY ? 0.0f : M;
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-            for (uint32_t k = 0; k < parts; k++) {
-              const float2 e = __ldcg(reinterpret_cast<const float2 *>(part(k) + HD));
-              const float4 v = __ldcg(reinterpret_cast<const float4 *>(part(k) + d));
-              const float f = ex2(e.x - base);
-              L = fmaf(f, e.y, L);
-              acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
+            for (uint32_t k0 = 0; k0 < parts; k0 += QUADS) {  // the lanes of a head: a part each
+              const uint32_t mine_k = k0 + lane % QUADS, n = min(QUADS, parts - k0);
+              const float2 e = mine_k < parts ? __ldcg(reinterpret_cast<const float2 *>(part(mine_k) + HD)) : make_float2(-INFINITY, 0.0f);
+              float old = 1.0f, f = 0.0f;
+              for (uint32_t q0 = 0; q0 < n; q0 += FLIGHT) {
+                float4 v[FLIGHT];
+#pragma unroll
+                for (uint32_t q = 0; q < FLIGHT; q++)
+                  v[q] = q0 + q < n ? __ldcg(reinterpret_cast<const float4 *>(part(k0 + q0 + q) + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                if (q0 == 0u) {  // (the first outputs are on their way by now)
+                  float m = e.x;
+#pragma unroll
+                  for (uint32_t o = 1; o < QUADS; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+                  const float M_new = fmaxf(M, m), base = M_new == -INFINITY ? 0.0f : M_new;
+                  old = ex2(M - base), f = ex2(e.x - base);
+                  float l = f * e.y;
+#pragma unroll
+                  for (uint32_t o = 1; o < QUADS; o <<= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
+                  L = fmaf(L, old, l), M = M_new;
+                  acc.x *= old, acc.y *= old, acc.z *= old, acc.w *= old;
+                }
+#pragma unroll
+                for (uint32_t q = 0; q < FLIGHT; q++) {
+                  const float w = __shfl_sync(0xFFFFFFFFu, f, lane / QUADS * QUADS + ((q0 + q) & (QUADS - 1u)));
+                  if (q0 + q < n) acc.x = fmaf(w, v[q].x, acc.x), acc.y = fmaf(w, v[q].y, acc.y), acc.z = fmaf(w, v[q].z, acc.z), acc.w = fmaf(w, v[q].w, acc.w);
+                }
+              }
             }
             const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
             acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
-            store_row4<HD>(a.out, a.out_stride, a.oq, a.oq_stride, a.wide, a.n_head * HD / 32u, c.r, h0 + h, d, acc, i < heads * QUADS);
+            store_row4<HD>(a.out, a.out_stride, a.oq, a.oq_stride, a.wide, a.n_head * HD / 32u, c.r, h0 + hh, d, acc, h < heads);
           }
         }
       }
-      x += c.j1 - c.j0;
-      if (c.left == 0u) break;
-      advance(c);
+      if (!go_on) break;
+      c = next;
       __syncthreads();  // everybody has read the records (and misc): the next unit's may be written
     }
     __pipeline_wait_prior(0);
@@ -501,24 +583,33 @@ __global__ void __launch_bounds__(AP_THREADS, ApGeom<KV, HD>::CTAS) attn_paged_k
       continue;
     }
     float *out = reinterpret_cast<float *>(reinterpret_cast<char *>(a.out) + a.out_stride * r);
-    for (uint32_t i = tid; i < a.n_head * HD; i += AP_THREADS) out[i] = 0.0f;
+    for (uint32_t i = tid; i < a.n_head * HD; i += THREADS) out[i] = 0.0f;
     if (a.oq)
-      for (uint32_t i = tid; i < a.n_head * HD / 32u * 10u; i += AP_THREADS) reinterpret_cast<uint32_t *>(a.oq + a.oq_stride * r)[i] = 0u;
+      for (uint32_t i = tid; i < a.n_head * HD / 32u * 10u; i += THREADS) reinterpret_cast<uint32_t *>(a.oq + a.oq_stride * r)[i] = 0u;
   }
 }
 
 constexpr size_t AP_COUNT_BYTES = AP_MAX_CTAS * 4u;
 static size_t ap_record_bytes(uint32_t hd) { return (size_t)AP_HEADS * (hd + 4u) * sizeof(float); }
 
-template <typename KV, int HD>
+template <typename KV, int HD, int W>
 static int launch_ap(PagedAttnArgs &a, cudaStream_t st) {
-  using Gm = ApGeom<KV, HD>;
-  auto k = attn_paged_kernel<KV, HD>;
+  using Gm = ApGeom<KV, HD, W>;
+  auto k = attn_paged_kernel<KV, HD, W>;
   if (int r = ensure_dynamic_smem(reinterpret_cast<const void *>(k), Gm::TOTAL)) return r;
   const uint32_t sms = (uint32_t)sm_count(), ctas = sms * Gm::CTAS < AP_MAX_CTAS ? sms * Gm::CTAS : AP_MAX_CTAS;
-  a.min_share = 256u / Gm::CH;
-  IEB_LAUNCH_PDL("attn_paged_kernel", k, dim3(ctas), dim3(AP_THREADS), Gm::TOTAL, st, a);
+  a.min_share = 128u / Gm::CH;  // 128 positions: 1 x 100 of 8 KV heads in 5.5 us (64: 7.5, 256: 5.5), 1 x 500 in 8.1 (8.0, 9.3)
+  IEB_LAUNCH_PDL("attn_paged_kernel", k, dim3(ctas), dim3(32 * W), Gm::TOTAL, st, a);
   return IE_B200_OK;
+}
+// Eight warps to a CTA, or four and twice the CTAs: eight where there are few units, whose parts are then longer and fewer to merge (1 x
+// 32768 positions of 8 KV heads 30.3 against 34.0 us, of 4 22.3 / 28.6; at 64 units, 8 x 1000, 14.5 / 14.2), and where they may be
+// long (64 x 8192 at most 92.0 / 93.8); four where a unit's end comes often (32 x 1000 29.6 / 27.6, 256 x 200 64 / 51) and, for its
+// arithmetic, with the float cache (64 x 3001 at most 158 / 145). What the host knows of the lengths is how wide the table is.
+template <typename KV, int HD>
+static int launch_ap(PagedAttnArgs &a, cudaStream_t st) {
+  const bool few = 2u * (uint64_t)a.R * a.kv.n_kv * a.groups <= (uint32_t)sm_count(), maybe_long = sizeof(KV) == 2 && table_positions(a.kv) >= 2048u;
+  return few || maybe_long ? launch_ap<KV, HD, 8>(a, st) : launch_ap<KV, HD, 4>(a, st);
 }
 
 }  // namespace ieb
