@@ -34,10 +34,11 @@ constexpr uint32_t SM_NONE = 0xFFFFFFFFu;
 struct SampleArgs {
   const float *x, *u, *temp, *top_p, *min_p;
   const uint32_t *top_k;
-  uint32_t *out;
+  uint32_t *idx;
+  float *prob;
   uint32_t n, slice, cl, wide;
   int frac;  // F
-  size_t x_stride, out_stride;
+  size_t x_stride;
 };
 
 // A CTA's shared memory in front of its slice (with the slice of 152064 logits over 8 CTAs: two CTAs on an SM).
@@ -136,8 +137,8 @@ __device__ __noinline__ uint64_t sm_weight(double diff, double c128) {
 }
 
 __device__ __forceinline__ void sample_out(const SampleArgs &a, uint32_t row, uint32_t idx, float prob) {
-  uint32_t *o = reinterpret_cast<uint32_t *>(reinterpret_cast<char *>(a.out) + a.out_stride * row);
-  o[0] = idx, o[1] = __float_as_uint(prob);
+  a.idx[row] = idx;
+  if (a.prob) a.prob[row] = prob;
 }
 // What a running sum of integers has to exceed to exceed u times the sum, and what it has to reach to reach p times the sum.
 __device__ __forceinline__ uint64_t sample_goal(float u, uint64_t all) {
@@ -693,16 +694,15 @@ static uint32_t sample_ctas(uint32_t n) { return n <= 4096u ? 1u : n <= 16384u ?
 
 using namespace ieb;
 
-extern "C" int ie_b200_sample(const float *d_x, uint32_t n, uint32_t *d_out, const float *d_u, const float *d_temp, const uint32_t *d_top_k, const float *d_top_p,
-                              const float *d_min_p, uint32_t T, size_t x_stride, size_t out_stride, void *stream) {
+extern "C" int ie_b200_sample(const float *d_x, uint32_t n, uint32_t *d_idx, float *d_prob, const float *d_u, const float *d_temp, const uint32_t *d_top_k,
+                              const float *d_top_p, const float *d_min_p, uint32_t T, size_t x_stride, void *stream) {
   if (T == 0) return IE_B200_OK;  // (an empty tensor may have no address)
-  if (!d_x || !d_out || !d_u) return fail(IE_B200_E_ARG, "ie_b200_sample: NULL pointer");
-  if (((uintptr_t)d_x | (uintptr_t)d_out | (uintptr_t)d_u | (uintptr_t)d_temp | (uintptr_t)d_top_k | (uintptr_t)d_top_p | (uintptr_t)d_min_p | x_stride | out_stride) & 3u)
+  if (!d_x || !d_idx || !d_u) return fail(IE_B200_E_ARG, "ie_b200_sample: NULL pointer");
+  if (((uintptr_t)d_x | (uintptr_t)d_idx | (uintptr_t)d_prob | (uintptr_t)d_u | (uintptr_t)d_temp | (uintptr_t)d_top_k | (uintptr_t)d_top_p | (uintptr_t)d_min_p | x_stride) & 3u)
     return fail(IE_B200_E_ARG, "ie_b200_sample: pointers and strides must be 4-byte aligned");
   if (n == 0 || n > SM_MAX_SLICE * SM_MAX_CL) return fail(IE_B200_E_SIZE, "ie_b200_sample: rows of %u logits (1 .. %u)", n, SM_MAX_SLICE * SM_MAX_CL);
-  if (T > (1u << 20) || (T > 1u && (x_stride < (size_t)n * 4u || out_stride < 8u)))
-    return fail(IE_B200_E_SIZE, "ie_b200_sample: %u rows (at most 2^20) %zu bytes apart, results %zu", T, x_stride, out_stride);
-  SampleArgs a = {d_x, d_u, d_temp, d_top_p, d_min_p, d_top_k, d_out, n, 0u, sample_ctas(n), 0u, 0, x_stride, out_stride};
+  if (T > (1u << 20) || (T > 1u && x_stride < (size_t)n * 4u)) return fail(IE_B200_E_SIZE, "ie_b200_sample: %u rows (at most 2^20) %zu bytes apart", T, x_stride);
+  SampleArgs a = {d_x, d_u, d_temp, d_top_p, d_min_p, d_top_k, d_idx, d_prob, n, 0u, sample_ctas(n), 0u, 0, x_stride};
   a.slice = ((n + a.cl - 1u) / a.cl + 3u) & ~3u;
   a.wide = (((uintptr_t)d_x | (T > 1u ? x_stride : 0u)) & 15u) == 0u;
   int log2n = 0;

@@ -306,8 +306,8 @@ int ie_b200_argmax(const float *d_x, uint32_t n, uint32_t *d_out, uint32_t T, si
 size_t ie_b200_topk_scratch_bytes(uint32_t nv, uint32_t K, uint32_t T);
 int ie_b200_topk(const float *d_x, uint32_t nv, uint32_t K, uint32_t T, size_t x_stride, float *d_val, uint32_t *d_idx, void *d_scratch, void *stream);
 
-/* The draw of the next token of each of T rows of logits (rows x_stride bytes apart): out {u32 index, f32 probability} per row, out_stride
- * bytes apart, as ie_b200_argmax. Per row, with w_i = exp((x_i - max x) / temp) and the tokens in the order of ie_b200_topk (value
+/* The draw of the next token of each of T rows of logits (rows x_stride bytes apart): d_idx[T], and its probability d_prob[T] (may be
+ * NULL). Per row, with w_i = exp((x_i - max x) / temp) and the tokens in the order of ie_b200_topk (value
  * falling, equal values smaller index first): the first top_k tokens (0, or n and more: all); of these the shortest run from the top whose
  * mass reaches top_p times their mass (1 and more: all; at least one token); of these the ones with w_i >= min_p (0 and less: all; above 1
  * counts as 1). Drawn is the first of them, by index, at which the running sum of w exceeds u times the sum of all (u below 0
@@ -317,8 +317,8 @@ int ie_b200_topk(const float *d_x, uint32_t nv, uint32_t K, uint32_t T, size_t x
  * probability 0; where the maximum is +inf its tokens are equally likely. d_u: T uniform numbers in [0, 1). d_temp, d_top_k, d_top_p,
  * d_min_p: T values each, or NULL (1, 0, 1, 0). n up to 360448. No scratch. The role of the reference's host sampler behind
  * backend.topk (src/gen.c, src/backend.h:33-37), which knows temp and top_k. */
-int ie_b200_sample(const float *d_x, uint32_t n, uint32_t *d_out, const float *d_u, const float *d_temp, const uint32_t *d_top_k, const float *d_top_p,
-                   const float *d_min_p, uint32_t T, size_t x_stride, size_t out_stride, void *stream);
+int ie_b200_sample(const float *d_x, uint32_t n, uint32_t *d_idx, float *d_prob, const float *d_u, const float *d_temp, const uint32_t *d_top_k,
+                   const float *d_top_p, const float *d_min_p, uint32_t T, size_t x_stride, void *stream);
 
 /* ie_b200_argmax for callers that cannot allocate device memory. It has no counterpart in the reference; it
  * exists for hosts that have already committed all device memory (arena and KV cache sized to fill the GPU at

@@ -83,13 +83,13 @@ def test_wrappers_refuse_what_is_not_on_a_gpu():
         K.attn_decode_paged(torch.zeros(1, 32), kp, kp, table, one, 1, None)
 
 
-def sample(lib, x=AT, n=1000, out=AT, u=AT, temp=None, k=None, p=None, m=None, T=1, x_stride=4000, out_stride=8):
-    return lib.ie_b200_sample(x, n, out, u, temp, k, p, m, T, x_stride, out_stride, None)
+def sample(lib, x=AT, n=1000, idx=AT, prob=AT, u=AT, temp=None, k=None, p=None, m=None, T=1, x_stride=4000):
+    return lib.ie_b200_sample(x, n, idx, prob, u, temp, k, p, m, T, x_stride, None)
 
 
-@pytest.mark.parametrize("change,status", [(dict(x=None), ARG), (dict(out=None), ARG), (dict(u=None), ARG), (dict(x=AT + 1), ARG), (dict(temp=AT + 2), ARG), (dict(k=AT + 2), ARG),
+@pytest.mark.parametrize("change,status", [(dict(x=None), ARG), (dict(idx=None), ARG), (dict(u=None), ARG), (dict(prob=AT + 2), ARG), (dict(x=AT + 1), ARG), (dict(temp=AT + 2), ARG), (dict(k=AT + 2), ARG),
                                            (dict(p=AT + 1), ARG), (dict(m=AT + 3), ARG), (dict(T=2, x_stride=4002), ARG), (dict(n=0), SIZE), (dict(n=360449), SIZE),
-                                           (dict(T=2, x_stride=3996), SIZE), (dict(T=2, out_stride=4), SIZE), (dict(T=(1 << 20) + 1), SIZE)])
+                                           (dict(T=2, x_stride=3996), SIZE), (dict(T=(1 << 20) + 1), SIZE)])
 def test_sample_refuses(lib, change, status):
     assert sample(lib, **change) == status and b"ie_b200_sample" in lib.ie_b200_last_error()
 
