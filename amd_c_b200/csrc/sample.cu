@@ -178,7 +178,8 @@ struct Sampler {
 #pragma unroll
     for (int e = 0; e < 4; e++) w[e] = distance(x[e]) <= none ? w[e] : 0u;
   }
-  __device__ __forceinline__ bool kept(float x, uint32_t i) const { return x > cut_x || (x == cut_x && i <= cut_idx); }
+  // (Here and in what the passes pick by: no && and ||, whose branches took longer than what they saved.)
+  __device__ __forceinline__ bool kept(float x, uint32_t i) const { return (x > cut_x) | ((x == cut_x) & (i <= cut_idx)); }
 
   // f(four logits, index of the first) for the tokens of this thread, in rising order
   template <typename F>
@@ -218,7 +219,7 @@ struct Sampler {
         const uint32_t i = begin + 4u * (qa + j);
         mask |= ((pred(v.x, i) ? 1u : 0u) | (pred(v.y, i + 1u) ? 2u : 0u) | (pred(v.z, i + 2u) ? 4u : 0u) | (pred(v.w, i + 3u) ? 8u : 0u)) << (4u * j);
       }
-      if (__any_sync(0xFFFFFFFFu, __popc(mask) > 6)) {
+      if (__any_sync(0xFFFFFFFFu, 2u * __popc(mask) > 3u * n)) {  // (four together take about as long as one and a half alone)
 #pragma unroll 1
         for (uint32_t j = 0; j < n; j++) {
           const float4 v = *reinterpret_cast<const float4 *>(xs + 4u * (qa + j));
@@ -385,7 +386,7 @@ struct Sampler {
     for (int round = 0; round < 5; round++) {
       const uint32_t w = round == 0 ? 0u : round == 4 ? 2u : 10u, last = round == 0 ? SM_BINS - 1u : (1u << w) - 1u;
       auto member = [&](float x, uint32_t i) {
-        return kept(x, i) && (round == 0 || (bin_of(x) == coarse && (bits == 0u || sm_key(x) >> (32u - bits) == prefix)));
+        return round == 0 ? kept(x, i) : kept(x, i) & (bin_of(x) == coarse) & ((uint32_t)((uint64_t)sm_key(x) >> (32u - bits)) == prefix);
       };
       auto bin = [&](float x) { return round == 0 ? bin_of(x) : last - ((sm_key(x) >> (32u - bits - w)) & last); };
       clear(last);
@@ -393,7 +394,7 @@ struct Sampler {
         each([&](const float (&x)[4], uint32_t i) {
 #pragma unroll
           for (uint32_t e = 0; e < 4; e++)
-            if (member(x[e], i + e)) count(bin(x[e]), 1u);
+            if (member(x[e], i + e)) atomicAdd(&s.low[bin(x[e])], 1u);
         });
       else if (round == 0 && cut_idx == SM_NONE) weigh_all([&](float x, uint32_t, uint64_t v) { count(bin_of(x), v); });
       else weigh(member, [&](float x, uint32_t, uint64_t v) { count(bin(x), v); });
@@ -418,7 +419,7 @@ struct Sampler {
           each([&](const float (&x)[4], uint32_t i) {
 #pragma unroll
             for (uint32_t e = 0; e < 4; e++)
-              if (bin_of(x[e]) <= b && kept(x[e], i + e)) add(x[e], i + e);
+              if ((bin_of(x[e]) <= b) & kept(x[e], i + e)) add(x[e], i + e);
           });
           const uint32_t n = gather();
           if (n <= (uint32_t)SM_THREADS) {
@@ -434,7 +435,7 @@ struct Sampler {
       each([&](const float (&x)[4], uint32_t i) {
 #pragma unroll
         for (uint32_t e = 0; e < 4; e++)
-          if (bin(x[e]) == b && member(x[e], i + e)) add(x[e], i + e);
+          if ((bin(x[e]) == b) & member(x[e], i + e)) add(x[e], i + e);
       });
       const uint32_t n = gather();
       above += ahead;
@@ -490,7 +491,7 @@ struct Sampler {
     // what is left are equal logits: as many of them as the goal takes, by index
     const float x = sm_unkey(prefix);
     const uint64_t w = MASS ? weight(x) : 1u, need = (goal - above + w - 1u) / w;
-    locate<false>([&](float y, uint32_t i) { return kept(y, i) && y == x; }, [&](uint64_t) { return need - 1u; },
+    locate<false>([&](float y, uint32_t i) { return kept(y, i) & (y == x); }, [&](uint64_t) { return need - 1u; },
                   [&](uint32_t idx, uint64_t, uint64_t) {
                     for (uint32_t c = 0; c < cl; c++) dsm_st32(peer(&s.base, c), idx);
                   });
@@ -539,7 +540,7 @@ struct Sampler {
 #pragma unroll
         for (uint32_t e = 0; e < 4; e++) {
           const bool in = pred(x[e], begin + 4u * q + e);
-          v[e] = MASS ? (in && v[e] >= least ? v[e] : 0u) : in;
+          v[e] = MASS ? (in & (v[e] >= least) ? v[e] : 0u) : in;
         }
       }
       const uint64_t four = (v[0] + v[1]) + (v[2] + v[3]), incl = warp_scan64(four, lane);
@@ -683,7 +684,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(const SampleArgs 
   }
   if (by_k) S.cut_run<false>(0.0f, top_k, u);
   if (by_p && S.cut_run<true>(top_p, 0u, u)) return;
-  S.locate<true>([&](float v, uint32_t i) { return S.distance(v) <= S.reach && S.kept(v, i); }, [&](uint64_t sum) { return sample_goal(u, sum); },
+  S.locate<true>([&](float v, uint32_t i) { return (S.distance(v) <= S.reach) & S.kept(v, i); }, [&](uint64_t sum) { return sample_goal(u, sum); },
                  [&](uint32_t idx, uint64_t w, uint64_t all) { sample_out(a, row, idx, (float)((double)w / (double)all)); });
 }
 
