@@ -36,7 +36,7 @@ struct SampleArgs {
   const uint32_t *top_k;
   uint32_t *idx;
   float *prob;
-  uint32_t n, slice, cl, wide;
+  uint32_t n, slice, cl, wide, sorted;
   int frac;  // F
   size_t x_stride;
 };
@@ -148,6 +148,26 @@ __device__ __forceinline__ uint64_t sample_goal(float u, uint64_t all) {
 __device__ __forceinline__ uint64_t run_goal(float p, uint64_t all) {
   const double g = ceil((double)p * (double)all);
   return g > 1.0 ? min(all, (uint64_t)g) : 1u;
+}
+
+// Where the rows are more than run at once: the i-th row of those that top_p makes long, then the i-th of the others (up to 512 rows).
+__device__ __forceinline__ uint32_t sample_row(const SampleArgs &a, uint32_t i) {
+  SampleSmem &s = sm_front();
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, T = gridDim.x / a.cl;
+  const uint32_t k = tid < T && a.top_k ? a.top_k[tid] : 0u;
+  const bool in = tid < T, is_long = in && a.top_p && a.top_p[tid] < 1.0f && (k == 0u || k > (uint32_t)SM_THREADS) && (!a.temp || a.temp[tid] > 0.0f);
+  const uint32_t longs = __ballot_sync(0xFFFFFFFFu, is_long);
+  if (lane == 0) s.wsum[warp] = __popc(longs);
+  __syncthreads();
+  uint32_t before = __popc(longs & ((1u << lane) - 1u)), all = 0u;
+  for (uint32_t w = 0; w < SM_WARPS; w++) {
+    const uint32_t n = (uint32_t)s.wsum[w];
+    if (w < warp) before += n;
+    all += n;
+  }
+  if (in && (is_long ? before : all + tid - before) == i) s.base = tid;
+  __syncthreads();
+  return s.base;
 }
 
 struct Sampler {
@@ -560,7 +580,8 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(const SampleArgs 
   float *xs = reinterpret_cast<float *>(smem_s + SM_FRONT);
   cluster_arrive();  // (waited for ahead of the first store into a peer, which has to run by then)
   pdl_prologue();
-  const uint32_t row = blockIdx.x / a.cl, rank = blockIdx.x % a.cl, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cl = a.cl;
+  const uint32_t rank = blockIdx.x % a.cl, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cl = a.cl;
+  const uint32_t row = a.sorted ? sample_row(a, blockIdx.x / a.cl) : blockIdx.x / a.cl;
   const uint32_t begin = min(a.n, rank * a.slice), count = min(a.n, begin + a.slice) - begin, quads = (count + 3u) / 4u;
 
   // ---- the slice; meanwhile the settings
@@ -703,7 +724,8 @@ extern "C" int ie_b200_sample(const float *d_x, uint32_t n, uint32_t *d_idx, flo
     return fail(IE_B200_E_ARG, "ie_b200_sample: pointers and strides must be 4-byte aligned");
   if (n == 0 || n > SM_MAX_SLICE * SM_MAX_CL) return fail(IE_B200_E_SIZE, "ie_b200_sample: rows of %u logits (1 .. %u)", n, SM_MAX_SLICE * SM_MAX_CL);
   if (T > (1u << 20) || (T > 1u && x_stride < (size_t)n * 4u)) return fail(IE_B200_E_SIZE, "ie_b200_sample: %u rows (at most 2^20) %zu bytes apart", T, x_stride);
-  SampleArgs a = {d_x, d_u, d_temp, d_top_p, d_min_p, d_top_k, d_idx, d_prob, n, 0u, sample_ctas(n), 0u, 0, x_stride};
+  SampleArgs a = {d_x, d_u, d_temp, d_top_p, d_min_p, d_top_k, d_idx, d_prob, n, 0u, sample_ctas(n), 0u, 0u, 0, x_stride};
+  a.sorted = d_top_p && T <= (uint32_t)SM_THREADS && T * a.cl > 2u * (uint32_t)sm_count();
   a.slice = ((n + a.cl - 1u) / a.cl + 3u) & ~3u;
   a.wide = (((uintptr_t)d_x | (T > 1u ? x_stride : 0u)) & 15u) == 0u;
   int log2n = 0;

@@ -100,6 +100,15 @@ def test_sample_without_settings(cuda):
     check(x, rng.random(9, dtype=np.float32), p=[0.6] * 9)
 
 
+@pytest.mark.parametrize("T,n", [(75, 50001), (512, 3000), (515, 700)])
+def test_sample_many_rows(cuda, T, n):
+    """More rows than run at once, of all kinds in turn: the long ones are taken first, and every row has its own result."""
+    rng = np.random.default_rng(T)
+    i = np.arange(T)
+    check(logits(rng, T, n), rng.random(T, dtype=np.float32), np.where(i % 7 == 3, 0.0, 0.5 + i % 5 * 0.3), np.where(i % 3 == 0, 5 + i % 40, 0) + np.where(i % 11 == 5, 600, 0),
+          np.where(i % 2 == 0, 0.9, 1.0), np.where(i % 4 == 1, 0.02, 0.0))
+
+
 @pytest.mark.parametrize("n", [10, 1000, 40000, 130000])
 def test_sample_equal_logits(cuda, n):
     """Logits that are all equal, or of a few values: the runs end inside ties, which go by index; every sum of equal weights is exact."""
