@@ -575,17 +575,21 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
     __pipeline_wait_prior(0);
   }
 
-  // ---- rows that see nothing: zeros
-  for (uint32_t r = blockIdx.x; r < a.R; r += gridDim.x) {
-    uint32_t seq;
-    if (ap_row(a, r, seq) != 0u || seq >= a.kv.n_seq) {
-      if (seq < a.kv.n_seq && a.err && tid == 0 && __ldg(a.len + r) > table_positions(a.kv)) atomicExch(a.err, ERR_PAGES);
-      continue;
+  // ---- rows that see nothing: zeros (a lane looks at a row, its warp writes it)
+  const uint32_t warps = gridDim.x * WARPS;
+  for (uint32_t r0 = blockIdx.x * WARPS + warp; r0 < a.R; r0 += 32u * warps) {
+    const uint32_t r = r0 + lane * warps;
+    uint32_t seq = 0xFFFFFFFFu, len = 1u;
+    if (r < a.R) len = ap_row(a, r, seq);
+    const bool real = r < a.R && seq < a.kv.n_seq;
+    if (real && a.err && __ldg(a.len + r) > len) atomicExch(a.err, ERR_PAGES);
+    for (uint32_t empty = __ballot_sync(0xFFFFFFFFu, real && len == 0u); empty; empty &= empty - 1u) {
+      const uint32_t e = r0 + (__ffs(empty) - 1u) * warps;
+      float *out = reinterpret_cast<float *>(reinterpret_cast<char *>(a.out) + a.out_stride * e);
+      for (uint32_t i = lane; i < a.n_head * HD; i += 32u) out[i] = 0.0f;
+      if (a.oq)
+        for (uint32_t i = lane; i < a.n_head * HD / 32u * 10u; i += 32u) reinterpret_cast<uint32_t *>(a.oq + a.oq_stride * e)[i] = 0u;
     }
-    float *out = reinterpret_cast<float *>(reinterpret_cast<char *>(a.out) + a.out_stride * r);
-    for (uint32_t i = tid; i < a.n_head * HD; i += THREADS) out[i] = 0.0f;
-    if (a.oq)
-      for (uint32_t i = tid; i < a.n_head * HD / 32u * 10u; i += THREADS) reinterpret_cast<uint32_t *>(a.oq + a.oq_stride * r)[i] = 0u;
   }
 }
 

@@ -12,11 +12,8 @@ constexpr uint32_t ERR_PAGES = 6u;  // error word: a length or position outside 
 int check_pages(const char *who, const ie_b200_kv_pages *p, uint32_t page_multiple);
 
 #ifdef __CUDACC__
-// Positions that the table can name.
-__host__ __device__ __forceinline__ uint32_t table_positions(const ie_b200_kv_pages &p) {
-  const uint64_t n = (uint64_t)p.table_cols * p.page;
-  return n < 0xFFFFFFFFull ? (uint32_t)n : 0xFFFFFFFFu;
-}
+// Positions that the table can name (below 2^31: check_pages).
+__host__ __device__ __forceinline__ uint32_t table_positions(const ie_b200_kv_pages &p) { return p.table_cols * p.page; }
 // The page number of column `col` of sequence `seq` (both inside the table).
 __device__ __forceinline__ uint32_t page_number(const ie_b200_kv_pages &p, uint32_t seq, uint32_t col) { return p.table[(size_t)seq * p.table_stride + col]; }
 // Byte offset, in either pool, of row `row` of KV head `head` in page `number`.

@@ -12,8 +12,9 @@ int check_pages(const char *who, const ie_b200_kv_pages *p, uint32_t page_multip
   if (!aligned16(p->kp) || !aligned16(p->vp) || (p->page_stride & 15u) || ((uintptr_t)p->table & 3u))
     return fail(IE_B200_E_ARG, "%s: pools and page stride must be 16-byte aligned, the table 4-byte", who);
   if (p->kv_f32 != 0 && p->kv_f32 != 1) return fail(IE_B200_E_ARG, "%s: kv_f32 %d is neither 0 nor 1", who, p->kv_f32);
-  if (!p->n_pages || !p->page || p->page % page_multiple || p->page > (1u << 20) || !p->n_kv || p->n_kv > 65535u || !p->table_cols || !p->n_seq)
-    return fail(IE_B200_E_SIZE, "%s: %u pages of %u positions (a multiple of %u), %u KV heads, a table of %u x %u", who, p->n_pages, p->page, page_multiple, p->n_kv,
+  if (!p->n_pages || !p->page || p->page % page_multiple || p->page > (1u << 20) || !p->n_kv || p->n_kv > 65535u || !p->table_cols || !p->n_seq ||
+      (uint64_t)p->table_cols * p->page > 0x7FFFFFFFull)
+    return fail(IE_B200_E_SIZE, "%s: %u pages of %u positions (a multiple of %u), %u KV heads, a table of %u x %u (at most 2^31 - 1 positions)", who, p->n_pages, p->page, page_multiple, p->n_kv,
                 p->n_seq, p->table_cols);
   if (p->hd == 0 || p->hd > 512u || p->hd % 8u) return fail(IE_B200_E_SIZE, "%s: head dim %u (a multiple of 8, at most 512)", who, p->hd);
   if (p->page_stride < (size_t)p->n_kv * p->page * p->hd * (p->kv_f32 ? 4u : 2u) || p->table_stride < p->table_cols)

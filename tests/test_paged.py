@@ -43,7 +43,7 @@ def test_the_packed_description_is_the_header_s():
 BAD_PAGES = [(dict(kp=None), ARG), (dict(vp=None), ARG), (dict(table=None), ARG), (dict(kp=AT + 8), ARG), (dict(vp=AT + 2), ARG), (dict(table=AT + 2), ARG),
              (dict(page_stride=16 * 8 * 128 * 2 + 8), ARG), (dict(kv_f32=2), ARG), (dict(n_pages=0), SIZE), (dict(page=0), SIZE), (dict(n_kv=0), SIZE),
              (dict(hd=0), SIZE), (dict(hd=100), SIZE), (dict(hd=1024), SIZE), (dict(n_seq=0), SIZE), (dict(table_cols=0), SIZE), (dict(table_stride=4), SIZE),
-             (dict(page_stride=16 * 8 * 128 * 2 - 16), SIZE), (dict(kv_f32=1), SIZE)]
+             (dict(page_stride=16 * 8 * 128 * 2 - 16), SIZE), (dict(kv_f32=1), SIZE), (dict(table_cols=1 << 27, table_stride=1 << 27), SIZE)]
 
 
 @pytest.mark.parametrize("change,status", BAD_PAGES)

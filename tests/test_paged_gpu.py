@@ -243,6 +243,23 @@ def test_attn_decode_paged_pages_that_do_not_exist(cuda, dtype):
     check_attention(out, None, *attention(q[2:], kp, vp, whole[2:3], [64], 4))
 
 
+def test_attn_decode_paged_many_rows_most_of_them_empty(cuda):
+    """More rows than the GPU has warps: rows of nothing are zeros wherever they lie, padding keeps what it had."""
+    q, kp, vp, table, _ = case(12, [33, 70], 4, 2, 64, 16, torch.half)
+    R = 5000
+    gen = torch.Generator().manual_seed(0)
+    seq, lens = torch.randint(-1, 2, (R,), generator=gen).int().to(cuda), torch.zeros(R, dtype=torch.int32, device=cuda)
+    some = torch.randperm(R, generator=gen)[:300].to(cuda)
+    lens[some] = torch.randint(1, 34, (300,), generator=gen).int().to(cuda)
+    q = torch.randn(R, 4 * 64, device=cuda, generator=generator(13))
+    out = torch.full_like(q, 5.0)
+    _, oq = K.attn_decode_paged(q, kp, vp, table, lens, 4, K.PagedScratch(4, 2, 64, cuda), seq=seq, out=out)
+    real, empty = seq >= 0, lens == 0
+    assert (out[~real] == 5).all() and (out[real & empty] == 0).all() and (oq[real & empty] == 0).all()
+    full = real & ~empty
+    check_attention(out[full], oq[full], *attention(q[full], kp, vp, table, lens[full], 4, seq[full]))
+
+
 def test_attn_decode_paged_strides(cuda):
     """Rows of q and of the output apart and off their 16-byte alignment; layers interleaved in one pool; a table that is a slice."""
     q, kp, vp, table, n = case(8, [77, 300], 6, 2, 64, 16, torch.half)
