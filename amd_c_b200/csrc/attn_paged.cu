@@ -297,6 +297,9 @@ struct ApCursor {
   uint64_t left, first;  // chunk numbers left behind j1; number of the unit's first chunk
 };
 
+// (A 64-bit division takes some 500 cycles.)
+__device__ __forceinline__ uint64_t ap_div(uint64_t x, uint64_t y) { return ((x | y) >> 32) == 0u ? (uint32_t)x / (uint32_t)y : x / y; }
+
 // Positions and sequence of row r: 0 positions where the row pads the batch.
 __device__ __forceinline__ uint32_t ap_row(const PagedAttnArgs &a, uint32_t r, uint32_t &seq) {
   seq = a.seq ? __ldg(a.seq + r) : r;
@@ -348,19 +351,22 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
     const uint32_t lc = chunks(r);
     mine += lc ? lc + END : 0u;
   }
-  uint64_t all = block_sum(mine, before) * units, share = (all + gridDim.x - 1u) / gridDim.x;
+  uint64_t all = block_sum(mine, before) * units, share = ap_div(all + gridDim.x - 1u, gridDim.x);
   if (share < a.min_share) share = a.min_share;
   uint32_t whole_shares = 1u;  // more: unit lengths are rounded up to a multiple of this
-  if ((uint64_t)a.R * units <= gridDim.x) {
-    for (uint32_t more = 0; more <= 3u * WARPS / 2u; more += WARPS / 4u) {
-      const uint32_t s = (uint32_t)share + more;
-      uint64_t parts = 0u, ahead;
-      for (uint32_t r = r_lo; r < r_hi; r++) parts += (chunks(r) + s - 1u) / s;
-      const uint64_t all_parts = block_sum(parts, ahead) * units;
-      if (all_parts <= gridDim.x) {
-        share = whole_shares = s, all = all_parts * s, before = ahead * s, mine = parts * s;
-        break;
-      }
+  if ((uint64_t)a.R * units <= gridDim.x) {  // a warp tries a length
+    const uint32_t s = (uint32_t)share + 2u * warp;
+    uint32_t parts = 0u;
+    for (uint32_t r = lane; r < a.R; r += 32u) parts += (chunks(r) + s - 1u) / s;
+    parts = __reduce_add_sync(0xFFFFFFFFu, parts);
+    if (lane == 0) misc[20 + warp] = parts * units <= gridDim.x ? s : 0xFFFFFFFFu;
+    __syncthreads();
+    uint32_t best = 0xFFFFFFFFu;
+    for (uint32_t w = 0; w < WARPS; w++) best = min(best, misc[20 + w]);
+    if (best != 0xFFFFFFFFu) {
+      mine = 0u;
+      for (uint32_t r = r_lo; r < r_hi; r++) mine += (chunks(r) + best - 1u) / best;
+      share = whole_shares = best, all = block_sum(mine, before) * units * best, before *= best, mine *= best;
     }
   }
   before *= units, mine *= units;
@@ -385,7 +391,7 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
       c.len = ap_row(a, c.r, c.seq);
       const uint32_t lc = (c.len + CH - 1u) / CH, num = numbered(lc);
       const uint64_t at = misc64[9];
-      c.unit = (uint32_t)(at / num), c.j0 = (uint32_t)(at - (uint64_t)c.unit * num);
+      c.unit = (uint32_t)ap_div(at, num), c.j0 = (uint32_t)(at - (uint64_t)c.unit * num);
       c.first = x0 - c.j0;
       const uint64_t end = min(c.first + num, x1);  // of the share's numbers in this unit
       c.left = x1 - end, c.j1 = (uint32_t)min((uint64_t)lc, end - c.first);
@@ -514,16 +520,16 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
         // The parts of the unit, in the order of its positions: the second record of the CTA it starts in, then the first ones of the
         // CTAs behind. Whoever is the last to have written adds them up.
         const uint64_t u0 = c.first;
-        const uint32_t c0 = (uint32_t)(u0 / share), parts = (uint32_t)((u0 + lc - 1u) / share) - c0 + 1u;
+        const uint32_t c0 = (uint32_t)ap_div(u0, share), parts = (uint32_t)ap_div(u0 + lc - 1u, share) - c0 + 1u;
         __threadfence();
         __syncthreads();
         if (tid == 0) {
           const bool last = atomicAdd(&a.count[c0], 1u) == parts - 1u;
           if (last) a.count[c0] = 0u;  // left zero for the next launch
-          misc[20] = last;
+          misc[30] = last;
         }
         __syncthreads();
-        if (misc[20]) {
+        if (misc[30]) {
           __threadfence();
           // A warp per head, or per several heads of fewer than 128 dims: the lanes share out the parts' (max, sum) and their weights, then
           // FLIGHT parts at a time are on their way.

@@ -601,9 +601,9 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(const SampleArgs 
   const float temp = a.temp ? a.temp[row] : 1.0f, top_p = a.top_p ? a.top_p[row] : 1.0f, min_p = a.min_p ? a.min_p[row] : 0.0f, u = a.u[row];
   const uint32_t top_k = a.top_k ? a.top_k[row] : 0u;
   const bool greedy = !(temp > 0.0f), by_k = !greedy && top_k > 0u && top_k < a.n, by_p = top_p < 1.0f;  // (a NaN: off)
-  const double c128 = greedy ? 0.0 : 184.6649652337873 / (double)temp;  // 128 log2(e) / temp
+  const double c128 = greedy ? 0.0 : 184.6649652337873 / (double)fmaxf(temp, 1.17549435e-38f);  // 128 log2(e) / temp (below 2^-126: as that, so that it fits in 32 bits)
   const float mp = min_p > 0.0f ? fminf(min_p, 1.0f) : 0.0f, none = (float)(a.frac + 1);
-  Sampler S = {a, s, xs, row, rank, cl, begin, quads, ((quads + SM_THREADS - 1u) / SM_THREADS) | 1u, 0.0f, (float)fmin(c128 / 128.0, 3.4e38), none,
+  Sampler S = {a, s, xs, row, rank, cl, begin, quads, ((quads + SM_THREADS - 1u) / SM_THREADS) | 1u, 0.0f, (float)(c128 / 128.0), none,
                fminf(none, mp > 0.0f ? 0.01f - log2f(mp) : none), 0.0, c128, max((uint64_t)1u, (uint64_t)ceil((double)mp * (double)(1ull << a.frac))), -INFINITY,
                SM_NONE, tid, warp, lane};
   if (tid < SM_TABLE && !greedy) s.pow2[tid] = scalbn(exp2((double)tid / SM_TABLE), a.frac);

@@ -312,11 +312,12 @@ int ie_b200_topk(const float *d_x, uint32_t nv, uint32_t K, uint32_t T, size_t x
  * falling, equal values smaller index first): the first top_k tokens (0, or n and more: all); of these the shortest run from the top whose
  * mass reaches top_p times their mass (1 and more: all; at least one token); of these the ones with w_i >= min_p (0 and less: all; above 1
  * counts as 1). Drawn is the first of them, by index, at which the running sum of w exceeds u times the sum of all (u below 0
- * counts as 0, 1 and more as just below 1); the probability is w_i over that sum. temp 0 (or less, or NaN): the first maximum, probability 1. Weights are
- * integers of 2^-44 of the largest one (2^-43 above 2^18 tokens; finer for shorter rows), their sums exact; a token whose weight rounds to
- * 0 is not drawn. A NaN logit is never drawn, one of -inf neither; a row with nothing else gives index 0xFFFFFFFF and
- * probability 0; where the maximum is +inf its tokens are equally likely. d_u: T uniform numbers in [0, 1). d_temp, d_top_k, d_top_p,
- * d_min_p: T values each, or NULL (1, 0, 1, 0). n up to 360448. No scratch. The role of the reference's host sampler behind
+ * counts as 0, 1 and more as just below 1); the probability is w_i over that sum. temp 0 (or less, or NaN): the first maximum,
+ * probability 1; a temp below 2^-126 counts as that. Weights are integers of 2^-44 of the largest one (2^-43 above 2^18 tokens; finer
+ * for shorter rows), their sums exact; a token whose weight rounds to 0 is not drawn. A NaN logit is never drawn, one of -inf neither,
+ * nor one that is further from the maximum than a float reaches; a row with nothing else gives index 0xFFFFFFFF and probability 0; where
+ * the maximum is +inf its tokens are equally likely. d_u: T uniform numbers in [0, 1). d_temp, d_top_k, d_top_p, d_min_p: T values
+ * each, or NULL (1, 0, 1, 0). n up to 360448, T up to 2^20. No scratch. The role of the reference's host sampler behind
  * backend.topk (src/gen.c, src/backend.h:33-37), which knows temp and top_k. */
 int ie_b200_sample(const float *d_x, uint32_t n, uint32_t *d_idx, float *d_prob, const float *d_u, const float *d_temp, const uint32_t *d_top_k,
                    const float *d_top_p, const float *d_min_p, uint32_t T, size_t x_stride, void *stream);
