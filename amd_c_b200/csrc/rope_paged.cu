@@ -3,6 +3,8 @@
 //
 // y_a = x_a c - x_b s, y_b = x_a s + x_b c for each pair (a, b) of dimensions and the table row of the token's position, every
 // product and sum rounded on its own (the bits of rope_kv_kernel in glue.cu and of the CPU path).
+// Bound: HBM for many tokens (8192 of 32 x 8 heads of 128, half pools: 58.5 us, 6.3 TB/s, 97 % of the measured copy rate), latency for few
+// (1: 2.0 us; 64: 2.3). A CTA per token keeps its table row and page number in registers for all its heads.
 #include "paged.cuh"
 
 namespace ieb {

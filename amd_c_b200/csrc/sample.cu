@@ -20,6 +20,8 @@
 //    atomics took 150 us at 1 x 128256, 720 at 64 x 152064). A short run of top-p goes to the first CTA whole, as above; of a long one
 //    the bin on the border does, or, where that holds too many, is split further by the bits of the logits until what is left are
 //    equal ones, which are counted off by index.
+// Measured (one row of 128256 / 64 rows of 152064, us): temp 0 3.7 / 13.5, top-k 50 8.3 / 26, no filter 8.0 / 32, min-p 6.6 / 24, top-p 0.9 16 / 60,
+// top-k 1000 16 / 49, top-p 0.95 of a flat row 25 / 94, a batch with all kinds 39.
 #include <cuda_pipeline_primitives.h>
 #include <math.h>
 

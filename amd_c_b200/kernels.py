@@ -298,6 +298,9 @@ def argmax(x: torch.Tensor) -> torch.Tensor:
 # ---- many sequences: a paged KV cache, attention over it, the draw of the next tokens. These take tensors of a server's own
 # making, so they look at them first; the work goes to the tensors' device, on its current stream. A decode step of one token is host
 # time, so what is usual is passed by one expression per tensor and only what fails it is looked at closely.
+_F32, _F16, _I32 = torch.float32, torch.float16, torch.int32
+
+
 def _refuse(name: str, t, dtype, shape, dev: int, what: str) -> None:
     got = f"{t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
     raise ValueError(f"{name}: want {dtype} {tuple('any' if n is None else n for n in shape)} on cuda:{dev}, {what}; got {got}")
@@ -326,7 +329,7 @@ def _rows(name: str, t: torch.Tensor, dtype, n: int | None, cols: int | None, de
 def _kv_pages(kp: torch.Tensor, vp: torch.Tensor, table: torch.Tensor) -> tuple[bytes, int, int, int, int]:
     """ie_b200_kv_pages of kp / vp [n_pages, n_kv, page, hd] half or float, pages any distance apart (alike in both), and a table
     [n_seq, columns] int32; with it the GPU, KV heads, head size and sequences."""
-    if not isinstance(kp, torch.Tensor) or kp.dim() != 4 or not kp.is_cuda or kp.dtype not in (torch.half, torch.float):
+    if not isinstance(kp, torch.Tensor) or kp.dim() != 4 or not kp.is_cuda or kp.dtype not in (_F16, _F32):
         raise ValueError("kp: want a half or float CUDA tensor [n_pages, n_kv, page, hd]")
     dev, dtype, shape, strides = kp.get_device(), kp.dtype, kp.shape, kp.stride()
     n, n_kv, page, hd = shape
@@ -337,8 +340,8 @@ def _kv_pages(kp: torch.Tensor, vp: torch.Tensor, table: torch.Tensor) -> tuple[
             if not isinstance(x, torch.Tensor) or x.dtype is not dtype or x.get_device() != dev or x.shape != shape or not n or not x[0].is_contiguous() or (
                     n > 1 and x.stride(0) != strides[0]):
                 _refuse(name, x, dtype, shape, dev, "each page contiguous, the pages of both as far apart")
-    size = 4 if dtype is torch.float else 2
-    at, n_seq, cols, stride = _rows("table", table, torch.int32, None, None, dev)
+    size = 4 if dtype is _F32 else 2
+    at, n_seq, cols, stride = _rows("table", table, _I32, None, None, dev)
     return (_lib.KV_PAGES.pack(kp.data_ptr(), vp.data_ptr(), at, n, page, n_kv, hd, n_seq, cols, stride, size == 4, (strides[0] if n > 1 else n_kv * own) * size),
             dev, n_kv, hd, n_seq)
 
@@ -357,7 +360,7 @@ def _run(fn, dev: int, args: tuple) -> None:
 
 def _seq(seq: torch.Tensor | None, n: int, n_seq: int, dev: int) -> int | None:
     if seq is not None:
-        return _flat("seq", seq, torch.int32, (n,), dev)
+        return _flat("seq", seq, _I32, (n,), dev)
     if n > n_seq:
         raise ValueError(f"{n} rows of their own sequences against a table of {n_seq}")
     return None
@@ -371,18 +374,18 @@ def rope_kv_paged(qkv: torch.Tensor, kp: torch.Tensor, vp: torch.Tensor, table: 
     pages, dev, kv_heads, kv_hd, n_seq = _kv_pages(kp, vp, table)
     if nkv != kv_heads or hd != kv_hd:
         raise ValueError(f"{nkv} KV heads of {hd} against pools of {kv_heads} heads of {kv_hd}")
-    base, T, _, step = _rows("qkv", qkv, torch.float, None, (nq + 2 * nkv) * hd, dev)
-    c, n_rope, half, row = _rows("cos", cos, torch.float, None, hd // 2, dev)
+    base, T, _, step = _rows("qkv", qkv, _F32, None, (nq + 2 * nkv) * hd, dev)
+    c, n_rope, half, row = _rows("cos", cos, _F32, None, hd // 2, dev)
     if row != half:
-        _refuse("cos", cos, torch.float, (None, half), dev, "contiguous")
-    s, p, q = _flat("sin", sin, torch.float, (n_rope, half), dev), _flat("pos", pos, torch.int32, (T,), dev), _seq(seq, T, n_seq, dev)
+        _refuse("cos", cos, _F32, (None, half), dev, "contiguous")
+    s, p, q = _flat("sin", sin, _F32, (n_rope, half), dev), _flat("pos", pos, _I32, (T,), dev), _seq(seq, T, n_seq, dev)
     if out is None:
-        out, out_step = torch.empty_strided((T, nq * hd), (nq * hd, 1), dtype=torch.float32, device=qkv.device), nq * hd  # (half the time of torch.empty)
+        out, out_step = torch.empty_strided((T, nq * hd), (nq * hd, 1), dtype=_F32, device=qkv.device), nq * hd  # (half the time of torch.empty)
         to = out.data_ptr()
     else:
-        to, _, _, out_step = _rows("out", out, torch.float, T, nq * hd, dev)
+        to, _, _, out_step = _rows("out", out, _F32, T, nq * hd, dev)
     _run(_lib.load().ie_b200_rope_kv_paged, dev, (base, base + 4 * nq * hd, base + 4 * (nq + nkv) * hd, to, pages, c, s, n_rope, p, q, nq, 1 if neox else 0, T, step * 4,
-                                                  out_step * 4, None if err is None else _flat("err", err, torch.int32, (1,), dev)))
+                                                  out_step * 4, None if err is None else _flat("err", err, _I32, (1,), dev)))
     return out
 
 
@@ -400,34 +403,34 @@ def attn_decode_paged(q: torch.Tensor, kp: torch.Tensor, vp: torch.Tensor, table
     sequence r). Returns (out [R, n_head hd], Q8 copies or None); a row that sees nothing is zeros, a row whose seq[r] is n_seq or
     more (-1 too) is left as it was."""
     pages, dev, n_kv, hd, n_seq = _kv_pages(kp, vp, table)
-    at, R, _, step = _rows("q", q, torch.float, None, n_head * hd, dev)
+    at, R, _, step = _rows("q", q, _F32, None, n_head * hd, dev)
     if scratch.layout != (n_head, n_kv, hd) or scratch.data.get_device() != dev:
         raise ValueError(f"scratch for {scratch.layout} (heads, KV heads, head size) on {scratch.data.device}, not {(n_head, n_kv, hd)} on cuda:{dev}")
-    n, sq, row, nbq = _flat("lens", lens, torch.int32, (R,), dev), _seq(seq, R, n_seq, dev), n_head * hd, n_head * hd // 32
+    n, sq, row, nbq = _flat("lens", lens, _I32, (R,), dev), _seq(seq, R, n_seq, dev), n_head * hd, n_head * hd // 32
     if out is None:
-        out, out_step = torch.empty_strided((R, row), (row, 1), dtype=torch.float32, device=q.device), row
+        out, out_step = torch.empty_strided((R, row), (row, 1), dtype=_F32, device=q.device), row
         to = out.data_ptr()
     else:
-        to, _, _, out_step = _rows("out", out, torch.float, R, row, dev)
+        to, _, _, out_step = _rows("out", out, _F32, R, row, dev)
     oq = torch.empty((R, q8_bytes(nbq)), dtype=torch.uint8, device=q.device) if quant else None
     _run(_lib.load().ie_b200_attn_decode_paged, dev, (at, pages, to, _p(oq), n, sq, n_head, R, step * 4, out_step * 4, q8_bytes(nbq), scratch.data.data_ptr(),
-                                                      None if err is None else _flat("err", err, torch.int32, (1,), dev)))
+                                                      None if err is None else _flat("err", err, _I32, (1,), dev)))
     return out, oq
 
 
 def sample(x: torch.Tensor, u: torch.Tensor, temp: torch.Tensor | None = None, top_k: torch.Tensor | None = None, top_p: torch.Tensor | None = None,
            min_p: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The next token of each row of logits x [T, n] f32, drawn with the uniform numbers u [T] f32: (indices int32 [T], probabilities f32
-    [T]). temp, top_p, min_p f32 [T] and top_k int32 [T] are each row's settings; None: 1, 1, 0, 0 (that filter off). A row
+    [T]). temp, top_p, min_p f32 [T] and top_k int32 [T] are each row's settings; None: that filter off (temp: 1). A row
     without a finite logit gives -1 and 0."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise ValueError("x: want a CUDA tensor [T, n]")
     dev = x.get_device()
-    at, T, n, step = _rows("x", x, torch.float, None, None, dev)
-    row, f32 = (T,), torch.float32
-    idx, prob = (torch.empty_strided(row, (1,), dtype=dt, device=x.device) for dt in (torch.int32, f32))
-    _run(_lib.load().ie_b200_sample, dev, (at, n, idx.data_ptr(), prob.data_ptr(), _flat("u", u, f32, row, dev),
-                                           None if temp is None else _flat("temp", temp, f32, row, dev), None if top_k is None else _flat("top_k", top_k, torch.int32, row, dev),
-                                           None if top_p is None else _flat("top_p", top_p, f32, row, dev),
-                                           None if min_p is None else _flat("min_p", min_p, f32, row, dev), T, step * 4))
+    at, T, n, step = _rows("x", x, _F32, None, None, dev)
+    row = (T,)
+    idx, prob = (torch.empty_strided(row, (1,), dtype=dt, device=x.device) for dt in (_I32, _F32))
+    _run(_lib.load().ie_b200_sample, dev, (at, n, idx.data_ptr(), prob.data_ptr(), _flat("u", u, _F32, row, dev),
+                                           None if temp is None else _flat("temp", temp, _F32, row, dev), None if top_k is None else _flat("top_k", top_k, _I32, row, dev),
+                                           None if top_p is None else _flat("top_p", top_p, _F32, row, dev),
+                                           None if min_p is None else _flat("min_p", min_p, _F32, row, dev), T, step * 4))
     return idx, prob
