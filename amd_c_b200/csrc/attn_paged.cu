@@ -40,8 +40,8 @@ struct PagedAttnArgs {
   const uint32_t *len, *seq;
   uint32_t *count, *err;
   ie_b200_kv_pages kv;
-  uint32_t n_head, G, groups, gw, R, wide;  // groups: head groups of a KV head, gw heads each (the last may have fewer)
-  uint32_t min_share;
+  uint32_t n_head, G, groups, gw, R, wide, seq0;  // groups: head groups of a KV head, gw heads each (the last may have fewer); seq0: sequence of row 0 where seq is NULL
+  uint32_t min_share, most;  // most: rows of a launch
   size_t q_stride, out_stride, oq_stride;
   float scale_log2;  // log2(e) / sqrt(hd)
 };
@@ -299,15 +299,12 @@ struct ApWarp<float, HD, W> {
 // Where a CTA's share stands: chunks [j, j1) of unit `unit` of row r (this share's part of it), and what is left behind them.
 struct ApCursor {
   uint32_t r, seq, len, unit, j0, j1;
-  uint64_t left, first;  // chunk numbers left behind j1; number of the unit's first chunk
+  uint32_t left, first;  // chunk numbers left behind j1; number of the unit's first chunk
 };
-
-// (A 64-bit division takes some 500 cycles.)
-__device__ __forceinline__ uint64_t ap_div(uint64_t x, uint64_t y) { return ((x | y) >> 32) == 0u ? (uint32_t)x / (uint32_t)y : x / y; }
 
 // Positions and sequence of row r: 0 positions where the row pads the batch.
 __device__ __forceinline__ uint32_t ap_row(const PagedAttnArgs &a, uint32_t r, uint32_t &seq) {
-  seq = a.seq ? __ldg(a.seq + r) : r;
+  seq = a.seq ? __ldg(a.seq + r) : r + a.seq0;
   return seq < a.kv.n_seq ? min(__ldg(a.len + r), table_positions(a.kv)) : 0u;
 }
 
@@ -321,7 +318,6 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
   uint8_t *ring = smem_ap + Gm::RING_OFF + warp * STAGES * Gm::STAGE;
   float *red = reinterpret_cast<float *>(smem_ap + Gm::RED_OFF), *ml = reinterpret_cast<float *>(smem_ap + Gm::ML_OFF);
   uint32_t *valid_of = reinterpret_cast<uint32_t *>(smem_ap + Gm::VALID_OFF) + warp * STAGES, *misc = reinterpret_cast<uint32_t *>(smem_ap + Gm::MISC_OFF);
-  uint64_t *misc64 = reinterpret_cast<uint64_t *>(misc);
   pdl_prologue();
   const uint32_t units = a.kv.n_kv * a.groups;
 
@@ -332,18 +328,19 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
     uint32_t seq;
     return (ap_row(a, r, seq) + CH - 1u) / CH;
   };
-  auto block_sum = [&](uint64_t mine, uint64_t &before) {  // of all threads, and of those ahead
-    uint64_t incl = mine, all = 0u;
+  auto block_sum = [&](uint32_t mine, uint32_t &before) {  // of all threads, and of those ahead
+    uint32_t incl = mine, all = 0u;
     for (int o = 1; o < 32; o <<= 1) {
-      const uint64_t v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+      const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
       if ((int)lane >= o) incl += v;
     }
     __syncthreads();
-    if (lane == 31) misc64[warp] = incl;
+    if (lane == 31) misc[warp] = incl;
     __syncthreads();
     before = incl - mine;
+#pragma unroll
     for (uint32_t w = 0; w < WARPS; w++) {
-      const uint64_t v = misc64[w];
+      const uint32_t v = misc[w];
       if (w < warp) before += v;
       all += v;
     }
@@ -351,16 +348,16 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
   };
   // Behind the chunks of a unit come some numbers without any, for what its end costs (about as long as a chunk of each warp).
   constexpr uint32_t END = WARPS;
-  uint64_t before, mine = 0u;
+  uint32_t before, mine = 0u;  // (chunk numbers fit in 32 bits: the launcher sees to it)
   for (uint32_t r = r_lo; r < r_hi; r++) {
     const uint32_t lc = chunks(r);
     mine += lc ? lc + END : 0u;
   }
-  uint64_t all = block_sum(mine, before) * units, share = ap_div(all + gridDim.x - 1u, gridDim.x);
+  uint32_t all = block_sum(mine, before) * units, share = (all + gridDim.x - 1u) / gridDim.x;
   if (share < a.min_share) share = a.min_share;
   uint32_t whole_shares = 1u;  // more: unit lengths are rounded up to a multiple of this
-  if ((uint64_t)a.R * units <= gridDim.x) {  // a warp tries a length
-    const uint32_t s = (uint32_t)share + 2u * warp;
+  if (a.R <= gridDim.x && a.R * units <= gridDim.x) {  // a warp tries a length
+    const uint32_t s = share + 2u * warp;
     uint32_t parts = 0u;
     for (uint32_t r = lane; r < a.R; r += 32u) parts += (chunks(r) + s - 1u) / s;
     parts = __reduce_add_sync(0xFFFFFFFFu, parts);
@@ -376,16 +373,15 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
   }
   before *= units, mine *= units;
   auto numbered = [&](uint32_t lc) { return whole_shares > 1u ? (lc + whole_shares - 1u) / whole_shares * whole_shares : lc ? lc + END : 0u; };  // of a unit of lc chunks
-  const uint64_t x0 = min(all, share * blockIdx.x), x1 = min(all, x0 + share);
+  const uint32_t x0 = min(all, share * blockIdx.x), x1 = min(all, x0 + share);
   if (x0 < x1 && before <= x0 && x0 < before + mine) {  // one thread
     uint32_t r = r_lo;
-    uint64_t row;
     for (;; r++) {
-      row = (uint64_t)numbered(chunks(r)) * units;
+      const uint32_t row = numbered(chunks(r)) * units;
       if (x0 < before + row) break;
       before += row;
     }
-    misc[16] = r, misc64[9] = x0 - before;  // row, chunk of the row
+    misc[16] = r, misc[17] = x0 - before;  // row, chunk of the row
   }
   __syncthreads();
 
@@ -395,11 +391,11 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
       c.r = misc[16];
       c.len = ap_row(a, c.r, c.seq);
       const uint32_t lc = (c.len + CH - 1u) / CH, num = numbered(lc);
-      const uint64_t at = misc64[9];
-      c.unit = (uint32_t)ap_div(at, num), c.j0 = (uint32_t)(at - (uint64_t)c.unit * num);
+      const uint32_t at = misc[17];
+      c.unit = at / num, c.j0 = at - c.unit * num;
       c.first = x0 - c.j0;
-      const uint64_t end = min(c.first + num, x1);  // of the share's numbers in this unit
-      c.left = x1 - end, c.j1 = (uint32_t)min((uint64_t)lc, end - c.first);
+      const uint32_t end = min(c.first + num, x1);  // of the share's numbers in this unit
+      c.left = x1 - end, c.j1 = min(lc, end - c.first);
     }
     auto advance = [&](ApCursor &k) {  // to the next unit (k.left > 0: there is one)
       k.first = x1 - k.left;
@@ -409,8 +405,8 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
         while (k.len == 0u);
       }
       const uint32_t lc = (k.len + CH - 1u) / CH;
-      const uint64_t end = min(k.first + numbered(lc), x1);
-      k.left = x1 - end, k.j0 = 0u, k.j1 = (uint32_t)min((uint64_t)lc, end - k.first);
+      const uint32_t end = min(k.first + numbered(lc), x1);
+      k.left = x1 - end, k.j0 = 0u, k.j1 = min(lc, end - k.first);
     };
     bool any = true;
     if (c.j0 >= c.j1) {  // the share starts behind the chunks of a unit
@@ -524,8 +520,7 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
       if (!whole) {
         // The parts of the unit, in the order of its positions: the second record of the CTA it starts in, then the first ones of the
         // CTAs behind. Whoever is the last to have written adds them up.
-        const uint64_t u0 = c.first;
-        const uint32_t c0 = (uint32_t)ap_div(u0, share), parts = (uint32_t)ap_div(u0 + lc - 1u, share) - c0 + 1u;
+        const uint32_t c0 = c.first / share, parts = (c.first + lc - 1u) / share - c0 + 1u;
         __threadfence();
         __syncthreads();
         if (tid == 0) {
@@ -614,7 +609,13 @@ static int launch_ap(PagedAttnArgs &a, cudaStream_t st) {
   if (int r = ensure_dynamic_smem(reinterpret_cast<const void *>(k), Gm::TOTAL)) return r;
   const uint32_t sms = (uint32_t)sm_count(), ctas = sms * Gm::CTAS < AP_MAX_CTAS ? sms * Gm::CTAS : AP_MAX_CTAS;
   a.min_share = 128u / Gm::CH;  // 128 positions: 1 x 100 of 8 KV heads in 5.5 us (64: 7.5, 256: 5.5), 1 x 500 in 8.1 (8.0, 9.3)
-  IEB_LAUNCH_PDL("attn_paged_kernel", k, dim3(ctas), dim3(32 * W), Gm::TOTAL, st, a);
+  for (uint32_t R = a.R; R;) {
+    a.R = R < a.most ? R : a.most;
+    IEB_LAUNCH_PDL("attn_paged_kernel", k, dim3(ctas), dim3(32 * W), Gm::TOTAL, st, a);
+    R -= a.R;
+    a.q = reinterpret_cast<const float *>(reinterpret_cast<const char *>(a.q) + a.q_stride * a.R), a.out = reinterpret_cast<float *>(reinterpret_cast<char *>(a.out) + a.out_stride * a.R);
+    a.oq = a.oq ? a.oq + a.oq_stride * a.R : nullptr, a.len += a.R, a.seq = a.seq ? a.seq + a.R : nullptr, a.seq0 += a.R;
+  }
   return IE_B200_OK;
 }
 // Eight warps to a CTA, or four and twice the CTAs: eight where there are few units, whose parts are then longer and fewer to merge (1 x
@@ -650,10 +651,15 @@ extern "C" int ie_b200_attn_decode_paged(const float *d_q, const ie_b200_kv_page
   const size_t row = (size_t)n_head * hd;
   if (R > (1u << 20) || (R > 1u && (q_stride < row * 4u || out_stride < row * 4u || (d_oq && oq_stride < row / 32u * 40u))))
     return fail(IE_B200_E_SIZE, "ie_b200_attn_decode_paged: %u rows (at most 2^20) with strides of %zu, %zu and %zu bytes", R, q_stride, out_stride, oq_stride);
+  // Chunk numbers of a launch stay below 2^31: a batch whose tables could hold more goes in several.
+  const uint32_t groups = (n_head / n_kv + AP_HEADS - 1u) / AP_HEADS;
+  const uint64_t numbers = ((uint64_t)table_positions(*pages) / (pages->kv_f32 ? 8u : 16u) + 9u) * n_kv * groups;
+  if (numbers >= (1ull << 31)) return fail(IE_B200_E_SIZE, "ie_b200_attn_decode_paged: tables of %u positions for %u KV heads", table_positions(*pages), n_kv);
   PagedAttnArgs a = {};
+  a.most = (uint32_t)(((1ull << 31) - 1u) / numbers);
   a.q = d_q, a.out = d_out, a.oq = static_cast<uint8_t *>(d_oq), a.len = d_len, a.seq = d_seq, a.err = d_err, a.kv = *pages;
   a.count = static_cast<uint32_t *>(d_scratch), a.rec = reinterpret_cast<float *>(static_cast<char *>(d_scratch) + AP_COUNT_BYTES);
-  a.n_head = n_head, a.G = n_head / n_kv, a.groups = (a.G + AP_HEADS - 1u) / AP_HEADS, a.gw = (a.G + a.groups - 1u) / a.groups, a.R = R;
+  a.n_head = n_head, a.G = n_head / n_kv, a.groups = groups, a.gw = (a.G + a.groups - 1u) / a.groups, a.R = R;
   a.wide = (((uintptr_t)d_out | out_stride) & 15u) == 0u;
   a.q_stride = q_stride, a.out_stride = out_stride, a.oq_stride = oq_stride;
   a.scale_log2 = 1.44269504088896340736f / sqrtf((float)hd);

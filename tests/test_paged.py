@@ -63,7 +63,8 @@ def test_rope_kv_paged_refuses(lib, change, status):
                                            (dict(q=AT + 4), ARG), (dict(q_stride=4096 * 4 + 4), ARG), (dict(out=AT + 2), ARG), (dict(oq=AT + 1), ARG), (dict(lens=AT + 2), ARG),
                                            (dict(scratch=AT + 8), ARG), (dict(p=pages(page=8, page_stride=1 << 20)), SIZE), (dict(p=pages(page=24, page_stride=1 << 20)), SIZE),
                                            (dict(p=pages(hd=96)), SIZE), (dict(n_head=30), SIZE), (dict(n_head=0), SIZE), (dict(R=2, q_stride=1024), SIZE),
-                                           (dict(R=2, out_stride=1024), SIZE), (dict(R=2, oq=AT, oq_stride=1024), SIZE), (dict(R=(1 << 20) + 1), SIZE)])
+                                           (dict(R=2, out_stride=1024), SIZE), (dict(R=2, oq=AT, oq_stride=1024), SIZE), (dict(R=(1 << 20) + 1), SIZE),
+                                           (dict(p=pages(n_kv=2048, page=1 << 20, table_cols=2000, table_stride=2000, page_stride=1 << 42), n_head=2048, q_stride=1 << 20, out_stride=1 << 20), SIZE)])
 def test_attn_decode_paged_refuses(lib, change, status):
     assert attn(lib, **{"p": pages(), **change}) == status and b"ie_b200_attn_decode_paged" in lib.ie_b200_last_error()
 

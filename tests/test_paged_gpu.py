@@ -260,6 +260,35 @@ def test_attn_decode_paged_many_rows_most_of_them_empty(cuda):
     check_attention(out[full], oq[full], *attention(q[full], kp, vp, table, lens[full], 4, seq[full]))
 
 
+@pytest.mark.parametrize("own", [True, False])
+def test_attn_decode_paged_wide_tables(cuda, own):
+    """Tables of 2^24 positions, of which little is in use: 300 rows are more than one launch numbers; rows of their own sequences, and rows that
+    name theirs."""
+    lens = [(i * 13) % 41 for i in range(300 if own else 3)]
+    gen = generator(14)
+    kp, vp, table = make_cache(gen, lens, 8, 32, 1024, torch.half, extra_cols=(1 << 14) - 1)
+    for s, n in enumerate(lens):
+        for pool in (kp, vp):
+            put(pool, table, s, torch.randn(n, 8, 32, device=cuda, generator=gen))
+    q = torch.randn(300, 8 * 32, device=cuda, generator=gen)
+    seq = None if own else (torch.arange(300, device=cuda, dtype=torch.int32) * 7) % 4 - 1
+    n = torch.tensor(lens, dtype=torch.int32, device=cuda) if own else torch.tensor(lens, dtype=torch.int32, device=cuda)[seq.long().clamp(min=0)]
+    before, out = K._lib.load().ie_b200_launch_count(), torch.full_like(q, 2.0)
+    _, oq = K.attn_decode_paged(q, kp, vp, table, n, 8, K.PagedScratch(8, 8, 32, cuda), seq=seq, out=out)
+    assert K._lib.load().ie_b200_launch_count() - before == 2
+    real = torch.ones(300, dtype=torch.bool, device=cuda) if own else seq >= 0
+    assert (out[~real] == 2).all()
+    check_attention(out[real], oq[real], *attention(q[real], kp, vp, table, n[real], 8, None if own else seq[real]))
+
+
+def test_attn_decode_paged_peaked(cuda):
+    """Scores in the hundreds: a row's weight on very few positions, the largest anywhere among the parts."""
+    for dtype in (torch.half, torch.float):
+        q, kp, vp, table, n = case(15, [700, 3000, 40], 8, 2, 128, 16, dtype)
+        out, oq = K.attn_decode_paged(q * 40, kp, vp, table, n, 8, K.PagedScratch(8, 2, 128, cuda))
+        check_attention(out, oq, *attention(q * 40, kp, vp, table, n, 8))
+
+
 def test_attn_decode_paged_strides(cuda):
     """Rows of q and of the output apart and off their 16-byte alignment; layers interleaved in one pool; a table that is a slice."""
     q, kp, vp, table, n = case(8, [77, 300], 6, 2, 64, 16, torch.half)
