@@ -6,7 +6,7 @@
 //
 // Work. A chunk is CH positions of one (row, KV head, head group); pages hold whole chunks, so a chunk is one contiguous run of K and
 // one of V. All chunks of the batch, in that order, are cut into even shares, one per CTA, wherever the cuts fall: the CTAs finish
-// together whatever the lengths are. A CTA finds its share by a prefix sum over the rows' lengths. Its four warps take the chunks of
+// together whatever the lengths are. A CTA finds its share by a prefix sum over the rows' lengths. Its four or eight warps take the chunks of
 // a unit (row, KV head, group) in turn; each warp has its own ring of buffers that it fills itself (cp.async, rows past the length
 // zero-filled) and its own running maximum, sum and outputs, so nothing in the stream waits for another warp, and the ring runs on into
 // the next unit while this one's records are merged. A unit that lies in one CTA is finished there; the parts of a cut one go to
@@ -19,7 +19,7 @@
 // Float cache: the same with fp32 FMAs, four lanes per position.
 //
 // Measured (half cache, heads of 128): 256 rows of 1000 positions, 32 x 8 heads, 164 us = 6.4 TB/s, 98 % of the measured copy rate; 64 rows of 1 to
-// 8192, 28 x 4, 91 us = 6.0 TB/s; 1 of 32768, 40 x 8, 30.2 us (the contiguous kernel of attn_decode.cu 34 us with 32 x 8), of which
+// 8192, 28 x 4, 91 us = 6.0 TB/s; 1 of 32768, 40 x 8, 29.8 us (the contiguous kernel of attn_decode.cu 34 us with 32 x 8), of which
 // 4 us are the start (length, page number, first rows: dependent round trips) and 4 the merge of 18 parts; 1 of 500, 8.1 us. Float cache, heads of
 // 128: 64 rows of up to 3001, 145 us = 5.8 TB/s.
 #include <cuda_pipeline_primitives.h>
@@ -50,7 +50,7 @@ struct PagedAttnArgs {
 template <typename KV, int HD, int W>
 struct ApGeom {
   static constexpr bool F16 = sizeof(KV) == 2;
-  static constexpr int THREADS = 32 * W, STAGES = HD == 32 ? 5 : HD == 128 ? 3 : W == 4 ? 4 : F16 ? 3 : 5;  // buffers of a warp
+  static constexpr int STAGES = HD == 32 ? 5 : HD == 128 ? 3 : W == 4 ? 4 : F16 ? 3 : 5;  // buffers of a warp
   static constexpr int CH = F16 ? 16 : 8;                       // positions of a chunk
   static constexpr int ROWB = HD * (int)sizeof(KV), PIECES = ROWB / 16, PER_LANE = CH * PIECES / 32;
   static constexpr int STAGE = 2 * CH * ROWB;                   // K rows, then V rows
