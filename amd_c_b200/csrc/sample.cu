@@ -20,8 +20,8 @@
 //    atomics took 150 us at 1 x 128256, 720 at 64 x 152064). A short run of top-p goes to the first CTA whole, as above; of a long one
 //    the bin on the border does, or, where that holds too many, is split further by the bits of the logits until what is left are
 //    equal ones, which are counted off by index.
-// Measured (one row of 128256 / 64 rows of 152064, us): temp 0 3.7 / 13.5, top-k 50 8.3 / 26, no filter 8.0 / 32, min-p 6.6 / 24, top-p 0.9 16 / 60,
-// top-k 1000 16 / 49, top-p 0.95 of a flat row 25 / 94, a batch with all kinds 39.
+// Measured (one row of 128256 / 64 rows of 152064, us): temp 0 3.8 / 13, top-k 50 8.3 / 26, no filter 8.2 / 32, min-p 6.4 / 20, top-p 0.9 15 / 57,
+// top-k 1000 16 / 50, top-p 0.95 of a flat row 26 / 95, a batch with all kinds 39.
 #include <cuda_pipeline_primitives.h>
 #include <math.h>
 
@@ -228,8 +228,9 @@ struct Sampler {
   // (Whole warps call it.) The same for those that pred(logit, index) picks: 32 looked at at a time, so that few of them cost few
   // exponentials, not one for every four tokens of which some lane wants one; where a lane has many, all 32 are weighed, four together, and
   // the others used with a weight of 0.
-  template <typename P, typename C>
-  __device__ __forceinline__ void weigh(P pred, C use) const {
+  // maybe(logit): false only where pred is false for it and every smaller one; it is asked of the largest of four.
+  template <typename M, typename P, typename C>
+  __device__ __forceinline__ void weigh(M maybe, P pred, C use) const {
     const uint32_t q1 = min((tid + 1u) * run, quads);
 #pragma unroll 1
     for (uint32_t g = 0; g < run; g += 8u) {  // (as often in every lane: they meet at its end)
@@ -239,7 +240,8 @@ struct Sampler {
       for (uint32_t j = 0; j < n; j++) {
         const float4 v = *reinterpret_cast<const float4 *>(xs + 4u * (qa + j));
         const uint32_t i = begin + 4u * (qa + j);
-        mask |= ((pred(v.x, i) ? 1u : 0u) | (pred(v.y, i + 1u) ? 2u : 0u) | (pred(v.z, i + 2u) ? 4u : 0u) | (pred(v.w, i + 3u) ? 8u : 0u)) << (4u * j);
+        if (maybe(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w))))
+          mask |= ((pred(v.x, i) ? 1u : 0u) | (pred(v.y, i + 1u) ? 2u : 0u) | (pred(v.z, i + 2u) ? 4u : 0u) | (pred(v.w, i + 3u) ? 8u : 0u)) << (4u * j);
       }
       if (__any_sync(0xFFFFFFFFu, 2u * __popc(mask) > 3u * n)) {  // (four together take about as long as one and a half alone)
 #pragma unroll 1
@@ -419,7 +421,7 @@ struct Sampler {
             if (member(x[e], i + e)) atomicAdd(&s.low[bin(x[e])], 1u);
         });
       else if (round == 0 && cut_idx == SM_NONE) weigh_all([&](float x, uint32_t, uint64_t v) { count(bin_of(x), v); });
-      else weigh(member, [&](float x, uint32_t, uint64_t v) { count(bin(x), v); });
+      else weigh([](float) { return true; }, member, [&](float x, uint32_t, uint64_t v) { count(bin(x), v); });
       border([&](uint64_t all) {
         if (MASS && round == 0) goal = run_goal(p, all);
         return goal - above;
@@ -439,6 +441,7 @@ struct Sampler {
         for (int i = 0; i < SM_WARPS; i++) about += s.max_of[i];
         if (about <= 400.0f) {
           each([&](const float (&x)[4], uint32_t i) {
+            if (bin_of(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]))) > b) return;
 #pragma unroll
             for (uint32_t e = 0; e < 4; e++)
               if ((bin_of(x[e]) <= b) & kept(x[e], i + e)) add(x[e], i + e);
@@ -531,7 +534,7 @@ struct Sampler {
     if (MASS && cut_idx == SM_NONE && reach == none) {  // everything is in
       weigh_all([&](float, uint32_t, uint64_t w) { sum += w; });
     } else if (MASS) {
-      weigh(pred, [&](float, uint32_t, uint64_t w) { sum += w >= least ? w : 0u; });
+      weigh([&](float x) { return cut_idx != SM_NONE || distance(x) <= reach; }, pred, [&](float, uint32_t, uint64_t w) { sum += w >= least ? w : 0u; });
     } else {
       each([&](const float (&x)[4], uint32_t i) {
 #pragma unroll
