@@ -362,6 +362,57 @@ def test_paged_decode_steps_in_a_graph(cuda):
     torch.cuda.current_stream().wait_stream(side)
 
 
+def test_paged_more_rows_than_a_grid_is_high(cuda):
+    """70 000 tokens and rows in one call each: every one is done, and in its own place."""
+    T, gen = 70000, generator(16)
+    kp, vp, table = make_cache(gen, [T], 1, 32, 64, torch.float)
+    cos, sin = rope_tables(T, 32)
+    qkv = torch.randn(T, 96, device=cuda, generator=gen)
+    pos = torch.randperm(T, device=cuda, generator=gen).int()
+    q = K.rope_kv_paged(qkv, kp, vp, table, cos, sin, pos, torch.zeros_like(pos), 1, 1, 32, True)
+    k, v = get(kp, table, 0, T)[:, 0], get(vp, table, 0, T)[:, 0]
+    want, size = rotated(qkv.double().view(T, 3, 32), cos[pos.long()], sin[pos.long()], True)
+    assert ((q.double() - want[:, 0]).abs() <= 2.001 * 2.0 ** -24 * size[:, 0]).all()
+    assert ((k[pos.long()].double() - want[:, 1]).abs() <= 2.001 * 2.0 ** -24 * size[:, 1]).all() and torch.equal(v[pos.long()], qkv[:, 64:])
+    lens = (pos % 4).int()
+    out, oq = K.attn_decode_paged(q, kp, vp, table, lens, 1, K.PagedScratch(1, 1, 32, cuda), seq=torch.zeros_like(pos))
+    x = (q.double() @ k[:3].double().T / 32 ** 0.5).masked_fill(torch.arange(3, device=cuda) >= lens[:, None], float("-inf"))
+    w = torch.where(lens[:, None] > 0, torch.softmax(x, 1), 0.0)
+    bound = ((q.double().abs() @ k[:3].double().abs().T / 32 ** 0.5).amax(1, keepdim=True) + 1) * v[:3].double().abs().max()
+    check_attention(out, None, (w @ v[:3].double())[:, None], bound[:, None])
+    assert torch.equal(oq, torch.cat([K.quant_q8(out[:T // 2]), K.quant_q8(out[T // 2:])]))  # (the quantiser takes 65 535 rows)
+
+
+def test_paged_calls_at_once(cuda):
+    """Two batches on two streams, each with its own scratch and pages, and a draw between them: the bits that they give one after the
+    other; the same scratch in two graphs, replayed in turn."""
+    sets = [case(20 + i, [900, 33, 2000, 0, 1], 8, 2, 64, 16, torch.half) for i in range(2)]
+    scratch = [K.PagedScratch(8, 2, 64, cuda) for _ in sets]
+    logits, u = torch.randn(5, 40000, device=cuda, generator=generator(22)), torch.rand(5, device=cuda)
+    want = [K.attn_decode_paged(q, kp, vp, table, n, 8, scratch[0])[0] for q, kp, vp, table, n in sets]
+    token = K.sample(logits, u)[0]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = [[], [], []]
+    for _ in range(20):
+        for i, (q, kp, vp, table, n) in enumerate(sets):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(K.attn_decode_paged(q, kp, vp, table, n, 8, scratch[i])[0])
+        with torch.cuda.stream(streams[2]):
+            got[2].append(K.sample(logits, u)[0])
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[i]) for i in range(2) for x in got[i]) and all(torch.equal(x, token) for x in got[2])
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in sets], [torch.zeros_like(w) for w in want]
+    for (q, kp, vp, table, n), graph, out in zip(sets, graphs, outs):
+        with torch.cuda.graph(graph):
+            K.attn_decode_paged(q, kp, vp, table, n, 8, scratch[0], quant=False, out=out)
+    for _ in range(10):
+        for graph in graphs:
+            graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for o, w in zip(outs, want))
+
+
 def test_paged_wrappers_refuse(cuda):
     q, kp, vp, table, n = case(11, [20], 4, 2, 64, 16, torch.half)
     sc = K.PagedScratch(4, 2, 64, cuda)

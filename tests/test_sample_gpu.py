@@ -155,6 +155,20 @@ def test_sample_extreme_settings(cuda):
         check(logits(rng, 16, n), np.float32(u), t, [k] * 16, p, m, ends=range(6, 11))
 
 
+def test_sample_more_rows_than_a_grid_is_high(cuda):
+    rng = np.random.default_rng(11)
+    T, n = 70000, 6
+    x, u = rng.standard_normal((T, n)).astype(np.float32), rng.random(T, dtype=np.float32)
+    w = np.exp(x.astype(np.float64) - x.max(1, keepdims=True))
+    run = np.cumsum(w, 1)
+    goal = u.astype(np.float64)[:, None] * run[:, -1:]
+    judge = np.abs(run - goal).min(1) > 2 * n * 2.0 ** -43.7
+    idx, prob = K.sample(torch.from_numpy(x).cuda(), torch.from_numpy(u).cuda())
+    want = (run > goal).argmax(1)
+    assert judge.sum() >= T - 10 and (idx.cpu().numpy() == want)[judge].all()
+    assert np.abs(prob.cpu().numpy() - (w / run[:, -1:])[np.arange(T), want])[judge].max() <= 2.0 ** -23
+
+
 def test_sample_is_the_inverse_of_the_running_sum(cuda):
     """u over a fine even grid draws every token as often as its probability says, give or take one."""
     rng = np.random.default_rng(7)
