@@ -473,7 +473,7 @@ struct Sampler {
           if (m > (uint32_t)SM_SHORT) {  // a histogram of the list first (a sort of 1024 takes 8000 cycles)
             auto fine = [&](float x) {
               if (round == 0) return min((uint32_t)(SM_BINS - 1), (uint32_t)fmaxf((distance(x) * 48.0f - ((float)b - 0.5f)) * (float)SM_BINS, 0.0f));
-              return 1023u - ((sm_key(x) << bits) >> 22);
+              return 1023u - ((uint32_t)((uint64_t)sm_key(x) << bits) >> 22);  // (bits may be 32: all are equal)
             };
             auto mass = [&](float x) { return MASS ? weight(x) : 1u; };
             __syncthreads();

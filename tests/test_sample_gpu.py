@@ -122,6 +122,14 @@ def test_sample_equal_logits(cuda, n):
     check(some, u, k=[0, 1, 3, 5, 9, n // 3, n - 2, min(n, 1500)] * 3, p=[1.0] * 8 + [0.7] * 8 + [0.33] * 8, m=[0.0] * 12 + [0.1] * 12)
 
 
+def test_sample_neighbouring_floats(cuda):
+    """Several hundred each of floats that differ in their last two bits: the border lies in the last split of the bits."""
+    rng = np.random.default_rng(12)
+    x = (np.float32(1.0) + rng.integers(0, 4, (12, 2800)).astype(np.float32) * np.float32(2.0 ** -23)).astype(np.float32)
+    x[6:, ::3] -= np.float32(3.0)
+    check(x, rng.random(12, dtype=np.float32), k=[513, 650, 800, 1300, 1500, 0] * 2, p=[1.0, 0.9, 1.0, 1.0, 0.7, 0.4] * 2)
+
+
 def test_sample_masked_and_infinite(cuda):
     """Tokens masked by -inf, by the lowest float, by NaN; rows with nothing left; +inf."""
     rng = np.random.default_rng(5)
