@@ -121,7 +121,7 @@ static int launch_rope_paged(const RopePagedArgs &a, int neox, uint32_t T, cudaS
   const uint32_t x = a.kv.hd / (2u * W), y = 256u / x, heads = a.nq + 2u * a.kv.n_kv;
   const uint32_t parts = (heads + y - 1u) / y;
   // Few tokens: a CTA for every 256 / x heads, so that no thread has more than one to do.
-  const uint32_t gy = T * parts <= 4u * (uint32_t)sm_count() ? parts : 1u;
+  const uint32_t gy = (uint64_t)T * parts <= 4u * (uint32_t)sm_count() ? parts : 1u;
   IEB_LAUNCH_PDL("rope_kv_paged_kernel", (rope_kv_paged_kernel<KV, W>), dim3(T, gy), dim3(x, y), 0, st, a, neox);
   return IE_B200_OK;
 }
