@@ -20,8 +20,8 @@
 //    atomics took 150 us at 1 x 128256, 720 at 64 x 152064). A short run of top-p goes to the first CTA whole, as above; of a long one
 //    the bin on the border does, or, where that holds too many, is split further by the bits of the logits until what is left are
 //    equal ones, which are counted off by index.
-// Measured (one row of 128256 / 64 rows of 152064, us): temp 0 3.8 / 13, top-k 50 8.3 / 26, no filter 8.2 / 32, min-p 6.4 / 20, top-p 0.9 15 / 57,
-// top-k 1000 16 / 50, top-p 0.95 of a flat row 26 / 95, a batch with all kinds 39.
+// Measured (one row of 128256 / 64 rows of 152064, us): temp 0 3.8 / 13, top-k 50 7.3 / 23, no filter 8.2 / 32, min-p 6.4 / 20, top-p 0.9 15 / 57,
+// top-k 1000 17 / 51, top-p 0.95 of a flat row 24 / 90, a batch with all kinds 39.
 #include <cuda_pipeline_primitives.h>
 #include <math.h>
 
@@ -31,6 +31,7 @@ namespace ieb {
 
 constexpr int SM_THREADS = 512, SM_WARPS = SM_THREADS / 32, SM_PER = 3, SM_BINS = SM_PER * SM_THREADS, SM_LIST = 1024, SM_SHORT = 256, SM_MAX_CL = 8, SM_TABLE = 128;
 constexpr uint32_t SM_MAX_SLICE = 45056;  // floats of a CTA's slice: 176 KB
+static_assert(SM_MAX_SLICE / 4u / SM_THREADS < 32u, "a thread's run is no longer than a warp is wide");
 constexpr uint32_t SM_NONE = 0xFFFFFFFFu;
 
 struct SampleArgs {
@@ -182,6 +183,7 @@ struct Sampler {
   uint64_t least;                        // what a weight has to have to be drawn: min_p in their units, 1
   float cut_x;                           // the last token of the run that is kept so far
   uint32_t cut_idx, tid, warp, lane;
+  bool dense;                            // the run has a fifth of the row or more
 
   __device__ __forceinline__ uint32_t peer(const void *p, uint32_t cta) const { return cluster_map_shared(p, cta); }
 
@@ -439,6 +441,7 @@ struct Sampler {
         __syncthreads();
         about = 0.0f;
         for (int i = 0; i < SM_WARPS; i++) about += s.max_of[i];
+        dense = about * 5.0f > (float)a.n;
         if (about <= 400.0f) {
           each([&](const float (&x)[4], uint32_t i) {
             if (bin_of(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]))) > b) return;
@@ -492,10 +495,25 @@ struct Sampler {
               if (fine(sm_unkey((uint32_t)(s.list[i] >> 32))) == s.bin) s.mine[atomicAdd(&s.n_mine, 1u)] = s.list[i];
             __syncthreads();
             m = s.n_mine;
-            for (uint32_t i = tid; i < m; i += SM_THREADS) s.list[i] = s.mine[i];
-            __syncthreads();
+            if (m > 32u) {
+              for (uint32_t i = tid; i < m; i += SM_THREADS) s.list[i] = s.mine[i];
+              __syncthreads();
+            }
           }
-          sort_falling(m);
+          if (n > (uint32_t)SM_SHORT && m <= 32u) {  // as a rule: one warp does it
+            if (warp == 0u) {
+              const uint64_t e = lane < m ? s.mine[lane] : 0u, v = lane < m ? (MASS ? weight(sm_unkey((uint32_t)(e >> 32))) : 1u) : 0u;
+              uint64_t before = at;
+              for (uint32_t j = 0; j < m; j++) {
+                const uint64_t o = __shfl_sync(0xFFFFFFFFu, e, j), w = __shfl_sync(0xFFFFFFFFu, v, j);
+                if (o > e) before += w;
+              }
+              if (lane < m && before < goal && goal <= before + v)  // one thread
+                for (uint32_t c = 0; c < cl; c++) dsm_st64(peer(&s.cut, c), e);
+            }
+            m = 0u;
+          }
+          if (m) sort_falling(m);
 #pragma unroll 1
           for (uint32_t i0 = 0; i0 < m; i0 += SM_THREADS) {  // at most two rounds
             uint64_t all;
@@ -533,6 +551,8 @@ struct Sampler {
     uint64_t sum = 0u, mine, all = 0u;
     if (MASS && cut_idx == SM_NONE && reach == none) {  // everything is in
       weigh_all([&](float, uint32_t, uint64_t w) { sum += w; });
+    } else if (MASS && dense) {  // (picking first: 10900 cycles for 36 tokens to a thread, so 8900)
+      weigh_all([&](float x, uint32_t i, uint64_t w) { sum += pred(x, i) & (w >= least) ? w : 0u; });
     } else if (MASS) {
       weigh([&](float x) { return cut_idx != SM_NONE || distance(x) <= reach; }, pred, [&](float, uint32_t, uint64_t w) { sum += w >= least ? w : 0u; });
     } else {
@@ -610,7 +630,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(const SampleArgs 
   const float mp = min_p > 0.0f ? fminf(min_p, 1.0f) : 0.0f, none = (float)(a.frac + 1);
   Sampler S = {a, s, xs, row, rank, cl, begin, quads, ((quads + SM_THREADS - 1u) / SM_THREADS) | 1u, 0.0f, (float)(c128 / 128.0), none,
                fminf(none, mp > 0.0f ? 0.01f - log2f(mp) : none), 0.0, c128, max((uint64_t)1u, (uint64_t)ceil((double)mp * (double)(1ull << a.frac))), -INFINITY,
-               SM_NONE, tid, warp, lane};
+               SM_NONE, tid, warp, lane, false};
   if (tid < SM_TABLE && !greedy) s.pow2[tid] = scalbn(exp2((double)tid / SM_TABLE), a.frac);
   if (tid == 0) s.n_mine = 0u, s.n_list = 0u;
   __pipeline_wait_prior(0);
@@ -683,9 +703,18 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(const SampleArgs 
   if (by_k && top_k <= (uint32_t)SM_THREADS) {
     // a lower bound of the k-th largest of the 512 maxima, bit by bit from the top, until less than a quarter more of them reach it
     const uint32_t key = sm_key(mx);
-    uint32_t low = 0u;
+    uint32_t low = 0u, bit = 1u << 31;
+    if ((uint32_t)__syncthreads_count(mx > -INFINITY) >= top_k) {  // the leading bits that all but those of -inf have in common are settled (8.3 -> 7.9 us, k 50)
+      const uint32_t wl = __reduce_min_sync(0xFFFFFFFFu, mx > -INFINITY ? key : 0xFFFFFFFFu);
+      if (lane == 0) s.wsum[warp] = wl;
+      __syncthreads();
+      const uint32_t least = __reduce_min_sync(0xFFFFFFFFu, lane < SM_WARPS ? (uint32_t)s.wsum[lane] : 0xFFFFFFFFu), diff = least ^ sm_key(xmax);
+      bit = diff ? 1u << (31 - __clz(diff)) : 0u;
+      low = least & ~(2u * bit - 1u);
+      if (!bit) low = least;
+    }
 #pragma unroll 1
-    for (uint32_t bit = 1u << 31; bit >= 1u << 8; bit >>= 1) {
+    for (; bit >= 1u << 8; bit >>= 1) {
       const uint32_t reached = (uint32_t)__syncthreads_count(key >= (low | bit));
       if (reached >= top_k) {
         low |= bit;
@@ -693,7 +722,20 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(const SampleArgs 
       }
     }
     const float floor_x = sm_unkey(max(low, 0x00800000u));  // (the lowest finite float: -inf is none)
-    if (own >= floor_x)
+    const uint32_t hits = __ballot_sync(0xFFFFFFFFu, own >= floor_x);
+    if (2u * __popc(hits) <= S.run) {  // the warp looks through the runs of the few threads that have some, a lane to a group of four (1 x 128256, k 50: 7.9 -> 7.3 us)
+#pragma unroll 1
+      for (uint32_t b = hits; b; b &= b - 1u) {
+        const uint32_t q = (warp * 32u + __ffs(b) - 1u) * S.run + lane;
+        if (lane < S.run && q < quads) {
+          const float4 y = *reinterpret_cast<const float4 *>(xs + 4u * q);
+          const float v[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            if (v[e] >= floor_x) S.add(v[e], begin + 4u * q + e);
+        }
+      }
+    } else if (own >= floor_x) {
       S.each([&](const float (&v)[4], uint32_t i) {
         if (fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])) >= floor_x) {
 #pragma unroll
@@ -701,6 +743,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(const SampleArgs 
             if (v[e] >= floor_x) S.add(v[e], i + e);
         }
       });
+    }
     const uint32_t n = S.gather();
     if (n <= (uint32_t)SM_LIST) {
       if (rank == 0u) S.finish(n, min(top_k, n), u, [&](uint64_t all) { return by_p ? run_goal(top_p, all) : all; });
