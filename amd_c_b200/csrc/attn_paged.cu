@@ -42,6 +42,7 @@ struct PagedAttnArgs {
   ie_b200_kv_pages kv;
   uint32_t n_head, G, groups, gw, R, wide, seq0;  // groups: head groups of a KV head, gw heads each (the last may have fewer); seq0: sequence of row 0 where seq is NULL
   uint32_t min_share, most;  // most: rows of a launch
+  uint32_t cpp, step_col, step_off;  // chunks of a page; a warp's step from chunk to chunk, in pages and chunks
   size_t q_stride, out_stride, oq_stride;
   float scale_log2;  // log2(e) / sqrt(hd)
 };
@@ -66,6 +67,11 @@ struct ApGeom {
   __device__ static __forceinline__ uint32_t at(uint32_t row, uint32_t piece) {
     const uint32_t x = F16 ? (HD == 32 ? (row >> 1) & 3u : row & 7u) : (row & 1u) * 4u;
     return row * ROWB + ((piece ^ x) * 16u);
+  }
+  // A lane's i-th piece (512 bytes from one to the next), from where its first one goes: the rows between are a power of two, above the lane's own row.
+  __device__ static __forceinline__ uint32_t step(uint32_t first, int i) {
+    const int row = 32 / PIECES * i;
+    return (first ^ (F16 ? (HD == 32 ? (row >> 1) & 3 : row & 7) : (row & 1) * 4) * 16u) + 512u * i;
   }
 };
 
@@ -415,9 +421,11 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
     }
 
     // ---- the ring: this warp's chunks, in the order in which they are worked on, STAGES - 1 ahead
-    ApCursor f = c;  // what is fetched
-    uint32_t fj = f.j0 + warp, f_num = 0u, f_stage = 0u;
-    const uint32_t cpp = a.kv.page / CH;
+    ApCursor f = c;  // what is fetched: chunk fj, in page column f_col of the sequence's row of the table f_row, chunk f_off of the page
+    uint32_t fj = f.j0 + warp, f_num = 0u, f_stage = 0u, f_col = fj / a.cpp, f_off = fj - f_col * a.cpp;
+    const uint32_t *f_row = nullptr;
+    size_t f_head = 0u;  // byte offset of the KV head in a page
+    auto enter = [&] { f_row = a.kv.table + (size_t)f.seq * a.kv.table_stride, f_head = (size_t)(f.unit / a.groups) * a.kv.page * Gm::ROWB; };
     bool more = any;
     auto find = [&] {  // the next chunk of this warp and its page number (needed only one chunk later: nobody waits for it)
       while (fj >= f.j1) {
@@ -426,34 +434,46 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
           return;
         }
         advance(f);
-        fj = warp;
+        enter();
+        fj = warp, f_col = warp / a.cpp, f_off = warp - f_col * a.cpp;
       }
-      f_num = page_number(a.kv, f.seq, fj / cpp);
+      f_num = f_row[f_col];
     };
+    const uint32_t to0 = Gm::at(lane / Gm::PIECES, lane % Gm::PIECES);
     auto fetch = [&] {
       if (more) {
         const bool there = f_num < a.kv.n_pages;
         const uint32_t valid = there ? min(CH, f.len - fj * CH) : 0u;
         if (!there && a.err && lane == 0) atomicExch(a.err, ERR_PAGES);
-        const size_t from = there ? page_row(a.kv, f_num, f.unit / a.groups, (fj % cpp) * CH, Gm::ROWB) : 0u;
+        const size_t from = (there ? (size_t)f_num * a.kv.page_stride + f_head + f_off * (uint32_t)(CH * Gm::ROWB) : 0u) + lane * 16u;
         const char *ks = static_cast<const char *>(a.kv.kp) + from, *vs = static_cast<const char *>(a.kv.vp) + from;
         uint8_t *st = ring + f_stage * Gm::STAGE;
+        if (valid == CH) {
 #pragma unroll
-        for (int i = 0; i < Gm::PER_LANE; i++) {
-          const uint32_t n = lane + 32u * i, row = n / Gm::PIECES, piece = n % Gm::PIECES, to = Gm::at(row, piece);
-          const bool in = row < valid;
-          const size_t src = in ? n * 16u : 0u;
-          __pipeline_memcpy_async(st + to, ks + src, 16, in ? 0 : 16);
-          __pipeline_memcpy_async(st + CH * Gm::ROWB + to, vs + src, 16, in ? 0 : 16);
+          for (int i = 0; i < Gm::PER_LANE; i++) {
+            const uint32_t to = Gm::step(to0, i);
+            __pipeline_memcpy_async(st + to, ks + 512 * i, 16);
+            __pipeline_memcpy_async(st + CH * Gm::ROWB + to, vs + 512 * i, 16);
+          }
+        } else {
+#pragma unroll 1
+          for (int i = 0; i < Gm::PER_LANE; i++) {
+            const uint32_t row = (lane + 32u * i) / Gm::PIECES, to = Gm::at(row, lane % Gm::PIECES);
+            const bool in = row < valid;  // (a row that is not is zeros; no address behind the last page)
+            const size_t src = in ? 512u * i : 0u;
+            __pipeline_memcpy_async(st + to, ks + src, 16, in ? 0 : 16);
+            __pipeline_memcpy_async(st + CH * Gm::ROWB + to, vs + src, 16, in ? 0 : 16);
+          }
         }
         if (lane == 0) valid_of[f_stage] = valid;
-        fj += WARPS;
+        fj += WARPS, f_col += a.step_col, f_off += a.step_off;
+        if (f_off >= a.cpp) f_off -= a.cpp, f_col++;
         find();
       }
       __pipeline_commit();
       f_stage = f_stage + 1u == STAGES ? 0u : f_stage + 1u;
     };
-    if (any) find();
+    if (any) enter(), find();
 #pragma unroll
     for (int i = 0; i < STAGES - 1; i++) fetch();
 
@@ -608,6 +628,7 @@ static int launch_ap(PagedAttnArgs &a, cudaStream_t st) {
   auto k = attn_paged_kernel<KV, HD, W>;
   if (int r = ensure_dynamic_smem(reinterpret_cast<const void *>(k), Gm::TOTAL)) return r;
   const uint32_t sms = (uint32_t)sm_count(), ctas = sms * Gm::CTAS < AP_MAX_CTAS ? sms * Gm::CTAS : AP_MAX_CTAS;
+  a.cpp = a.kv.page / Gm::CH, a.step_col = W / a.cpp, a.step_off = W % a.cpp;
   a.min_share = 128u / Gm::CH;  // 128 positions: 1 x 100 of 8 KV heads in 5.5 us (64: 7.5, 256: 5.5), 1 x 500 in 8.1 (8.0, 9.3)
   for (uint32_t R = a.R; R;) {
     a.R = R < a.most ? R : a.most;
