@@ -55,6 +55,7 @@ struct ApGeom {
   static constexpr int CH = F16 ? 16 : 8;                       // positions of a chunk
   static constexpr int ROWB = HD * (int)sizeof(KV), PIECES = ROWB / 16, PER_LANE = CH * PIECES / 32;
   static constexpr int STAGE = 2 * CH * ROWB;                   // K rows, then V rows
+  static constexpr bool PAIRS = F16 && HD <= 64 && STAGES >= 4;  // two chunks worked on at once, where they are short (256 x 1000 of 16 x 16 heads of 64 167 -> 161 us, of 8 x 4 of 32 32.2 -> 30.3)
   static constexpr int REC_ROW = HD + 4;                        // floats between the heads of a record in global memory: outputs, max, sum
   static constexpr int RING_OFF = 0, RED_OFF = W * STAGES * STAGE, ML_OFF = RED_OFF + W * AP_HEADS * HD * 4,
                        VALID_OFF = ML_OFF + W * AP_HEADS * 8, MISC_OFF = (VALID_OFF + W * STAGES * 4 + 15) / 16 * 16, TOTAL = MISC_OFF + 128,
@@ -126,51 +127,76 @@ struct ApWarp<__half, HD, W> {
     }
     m[0] = m[1] = -INFINITY, l[0] = l[1] = 0.0f;
   }
-  __device__ __forceinline__ void chunk(const uint8_t *stage, uint32_t valid, float scale_log2, int lane) {
-    const uint32_t kb = smem_u32(stage), vb = kb + Gm::CH * Gm::ROWB, lm = lane >> 3, lr = lane & 7, hq = lane >> 2;
-    float sl[4] = {0.f, 0.f, 0.f, 0.f}, s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+  // N chunks at once, each with `valid` positions
+  template <int N>
+  __device__ __forceinline__ void chunks(const uint8_t *const (&stage)[N], const uint32_t (&valid)[N], float scale_log2, int lane) {
+    const uint32_t lm = lane >> 3, lr = lane & 7, hq = lane >> 2;
+    float s[N][4], al[2];  // s[.][j]: position lane / 4, s[.][2 + j]: + 8, of head 2 (lane % 4) + j
+    float sl[N][4] = {}, s0[N][4] = {}, s1[N][4] = {};
 #pragma unroll
-    for (int k = 0; k < KS; k++) {
-      uint32_t a[4];  // (positions lo, dims lo), (positions hi, dims lo), (positions lo, dims hi), (positions hi, dims hi)
-      ap_ldsm4(a, kb + Gm::at((lm & 1) * 8 + lr, 2 * k + (lm >> 1)));
-      ap_mma(sl, a, ql[k][0], ql[k][1]);
-      if (k & 1) ap_mma(s1, a, qh[k][0], qh[k][1]);
-      else ap_mma(s0, a, qh[k][0], qh[k][1]);
-    }
-    float s[4], p[4], al[2];  // s[j]: position lane / 4, s[2 + j]: + 8, of head 2 (lane % 4) + j
+    for (int k = 0; k < KS; k++)
 #pragma unroll
-    for (int e = 0; e < 4; e++) s[e] = (s0[e] + s1[e]) + sl[e];
-    if (valid < 16u) {
-      if (hq >= valid) s[0] = s[1] = -INFINITY;
-      if (hq + 8u >= valid) s[2] = s[3] = -INFINITY;
+      for (int n = 0; n < N; n++) {
+        uint32_t a[4];  // (positions lo, dims lo), (positions hi, dims lo), (positions lo, dims hi), (positions hi, dims hi)
+        ap_ldsm4(a, smem_u32(stage[n]) + Gm::at((lm & 1) * 8 + lr, 2 * k + (lm >> 1)));
+        ap_mma(sl[n], a, ql[k][0], ql[k][1]);
+        if (k & 1) ap_mma(s1[n], a, qh[k][0], qh[k][1]);
+        else ap_mma(s0[n], a, qh[k][0], qh[k][1]);
+      }
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) s[n][e] = (s0[n][e] + s1[n][e]) + sl[n][e];
+      if (valid[n] < 16u) {
+        if (hq >= valid[n]) s[n][0] = s[n][1] = -INFINITY;
+        if (hq + 8u >= valid[n]) s[n][2] = s[n][3] = -INFINITY;
+      }
     }
 #pragma unroll
     for (int j = 0; j < 2; j++) {
-      float mx = fmaxf(s[j], s[2 + j]);
+      float mx = fmaxf(s[0][j], s[0][2 + j]);
+#pragma unroll
+      for (int n = 1; n < N; n++) mx = fmaxf(mx, fmaxf(s[n][j], s[n][2 + j]));
       mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 4));
       mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 8));
       mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 16));
       const float m_new = fmaxf(m[j], mx * scale_log2), base = m_new == -INFINITY ? 0.0f : m_new;
       al[j] = ex2(m[j] - base);
-      p[j] = ex2(fmaf(s[j], scale_log2, -base)), p[2 + j] = ex2(fmaf(s[2 + j], scale_log2, -base));
-      l[j] = fmaf(l[j], al[j], p[j] + p[2 + j]);  // (of this lane's positions: the lanes meet in finish())
+      float sum = 0.0f;
+#pragma unroll
+      for (int n = 0; n < N; n++) {  // from here on the weights
+        s[n][j] = ex2(fmaf(s[n][j], scale_log2, -base)), s[n][2 + j] = ex2(fmaf(s[n][2 + j], scale_log2, -base));
+        sum += s[n][j] + s[n][2 + j];
+      }
+      l[j] = fmaf(l[j], al[j], sum);  // (of this lane's positions: the lanes meet in finish())
       m[j] = m_new;
     }
-    uint32_t ph[2], pl[2];  // each 8 x 8 block [positions x heads] transposed into the B fragment [positions x heads]
-    ap_split2(p[0] * 0x1p15f, p[1] * 0x1p15f, ph[0], pl[0]);
-    ap_split2(p[2] * 0x1p15f, p[3] * 0x1p15f, ph[1], pl[1]);
+    uint32_t ph[N][2], pl[N][2];  // each 8 x 8 block [positions x heads] transposed into the B fragment [positions x heads]
 #pragma unroll
-    for (int e = 0; e < 2; e++) ph[e] = ap_movm_t(ph[e]), pl[e] = ap_movm_t(pl[e]);
+    for (int n = 0; n < N; n++) {
+      ap_split2(s[n][0] * 0x1p15f, s[n][1] * 0x1p15f, ph[n][0], pl[n][0]);
+      ap_split2(s[n][2] * 0x1p15f, s[n][3] * 0x1p15f, ph[n][1], pl[n][1]);
+#pragma unroll
+      for (int e = 0; e < 2; e++) ph[n][e] = ap_movm_t(ph[n][e]), pl[n][e] = ap_movm_t(pl[n][e]);
+    }
 #pragma unroll
     for (int u = 0; u < KS; u++) {
-      uint32_t a[4];  // transposed on load: (dims lo, positions lo), (dims hi, positions lo), (dims lo, positions hi), (dims hi, positions hi)
-      ap_ldsm4t(a, vb + Gm::at((lm >> 1) * 8 + lr, 2 * u + (lm & 1)));
       float c[4] = {0.f, 0.f, 0.f, 0.f};
-      ap_mma(c, a, pl[0], pl[1]);
-      ap_mma(c, a, ph[0], ph[1]);
+#pragma unroll
+      for (int n = 0; n < N; n++) {
+        uint32_t a[4];  // transposed on load: (dims lo, positions lo), (dims hi, positions lo), (dims lo, positions hi), (dims hi, positions hi)
+        ap_ldsm4t(a, smem_u32(stage[n]) + Gm::CH * Gm::ROWB + Gm::at((lm >> 1) * 8 + lr, 2 * u + (lm & 1)));
+        ap_mma(c, a, pl[n][0], pl[n][1]);
+        ap_mma(c, a, ph[n][0], ph[n][1]);
+      }
 #pragma unroll
       for (int e = 0; e < 4; e++) o[u][e] = fmaf(o[u][e], al[e & 1], c[e]);
     }
+  }
+  __device__ __forceinline__ void chunk(const uint8_t *stage, uint32_t valid, float scale_log2, int lane) {
+    const uint8_t *const st[1] = {stage};
+    const uint32_t v[1] = {valid};
+    chunks<1>(st, v, scale_log2, lane);
   }
   // this warp's record: red [heads][HD] outputs (2^15 times; red_at), ml [heads][2]
   __device__ __forceinline__ void finish(float *red, float *ml, int lane) {
@@ -494,7 +520,22 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
       uint32_t h0;
       const uint32_t heads = heads_of(c, h0);
       w.start(heads, reinterpret_cast<float *>(smem_ap + Gm::Q_OFF), tid);
-      for (uint32_t j = c.j0 + warp; j < c.j1; j += WARPS) {
+      uint32_t j = c.j0 + warp;
+      if constexpr (Gm::PAIRS) {
+        for (; j + WARPS < c.j1; j += 2u * WARPS) {
+          __pipeline_wait_prior(STAGES - 3);
+          __syncwarp();
+          const uint32_t second = stage + 1u == STAGES ? 0u : stage + 1u;
+          const uint8_t *const st[2] = {ring + stage * Gm::STAGE, ring + second * Gm::STAGE};
+          const uint32_t valid[2] = {valid_of[stage], valid_of[second]};
+          fetch();
+          w.template chunks<2>(st, valid, a.scale_log2, lane);
+          __syncwarp();
+          fetch();
+          stage = second + 1u == STAGES ? 0u : second + 1u;
+        }
+      }
+      for (; j < c.j1; j += WARPS) {
         __pipeline_wait_prior(STAGES - 2);
         __syncwarp();
         const uint32_t valid = valid_of[stage];
