@@ -19,9 +19,9 @@
 // Float cache: the same with fp32 FMAs, four lanes per position.
 //
 // Measured (half cache, heads of 128): 256 rows of 1000 positions, 32 x 8 heads, 164 us = 6.4 TB/s, 98 % of the measured copy rate; 64 rows of 1 to
-// 8192, 28 x 4, 91 us = 6.0 TB/s; 1 of 32768, 40 x 8, 29.8 us (the contiguous kernel of attn_decode.cu 34 us with 32 x 8), of which
+// 8192, 28 x 4, 91 us = 6.0 TB/s; 1 of 32768, 40 x 8, 29.3 us (the contiguous kernel of attn_decode.cu 34 us with 32 x 8), of which
 // 4 us are the start (length, page number, first rows: dependent round trips) and 4 the merge of 18 parts; 1 of 500, 8.1 us. Float cache, heads of
-// 128: 64 rows of up to 3001, 145 us = 5.8 TB/s.
+// 128: 64 rows of up to 3001, 132 us = 6.3 TB/s; of 64: 253 rows of 868 141 us = 6.4 TB/s.
 #include <cuda_pipeline_primitives.h>
 #include <math.h>
 
@@ -219,7 +219,7 @@ template <int HD, int W>
 struct ApWarp<float, HD, W> {
   using Gm = ApGeom<float, HD, 4>;
   static constexpr int DPL = HD / 32;  // output dims of a lane
-  float o[AP_HEADS][DPL], m[AP_HEADS], l[AP_HEADS];
+  float o[AP_HEADS][DPL], m[2], l[2];  // m, l: of heads lane % 4 and that + 4
   static constexpr int QPT = AP_HEADS * HD / (32 * W);
   float q[QPT];  // this thread's part of the next unit's q, on its way
   const float *qs;
@@ -236,17 +236,16 @@ struct ApWarp<float, HD, W> {
     for (int i = 0; i < QPT; i++) q_smem[tid + 32u * W * i] = q[i];
     __syncthreads();
 #pragma unroll
-    for (int h = 0; h < AP_HEADS; h++) {
-      m[h] = -INFINITY, l[h] = 0.0f;
+    for (int h = 0; h < AP_HEADS; h++)
 #pragma unroll
       for (int d = 0; d < DPL; d++) o[h][d] = 0.0f;
-    }
+    m[0] = m[1] = -INFINITY, l[0] = l[1] = 0.0f;
   }
   // H: heads worked on, 4 or 8 (half the arithmetic where the unit has no more than four)
   template <int H>
   __device__ __forceinline__ void chunk_of(uint8_t *stage, uint32_t valid, float scale_log2, int lane) {
     const uint32_t pos = lane >> 2, part = lane & 3;  // lane: a quarter of the dims of one position
-    float s[H], al[H];
+    float s[H];
 #pragma unroll
     for (int h = 0; h < H; h++) s[h] = 0.0f;
 #pragma unroll 4
@@ -259,32 +258,42 @@ struct ApWarp<float, HD, W> {
         s[h] = fmaf(x.x, k.x, s[h]), s[h] = fmaf(x.y, k.y, s[h]), s[h] = fmaf(x.z, k.z, s[h]), s[h] = fmaf(x.w, k.w, s[h]);
       }
     }
+    // The four lanes' parts meet, and the heads part: lane `part` is left with the scores of head `part` and, of eight, of part + 4 (with all heads in
+    // every lane, 253 x 868 of heads of 64 took 164 us for 141).
+    const bool odd = part & 1u, upper = part & 2u;
+    float t[H / 2];
 #pragma unroll
-    for (int h = 0; h < H; h++) {
-      s[h] += __shfl_xor_sync(0xFFFFFFFFu, s[h], 1);
-      s[h] += __shfl_xor_sync(0xFFFFFFFFu, s[h], 2);
-      if (pos >= valid) s[h] = -INFINITY;
-      float mx = s[h];
+    for (int i = 0; i < H / 2; i++) t[i] = (odd ? s[2 * i + 1] : s[2 * i]) + __shfl_xor_sync(0xFFFFFFFFu, odd ? s[2 * i] : s[2 * i + 1], 1);
+    float w_own[H / 4], al_own[H / 4];
+#pragma unroll
+    for (int i = 0; i < H / 4; i++) {
+      float x = (upper ? t[2 * i + 1] : t[2 * i]) + __shfl_xor_sync(0xFFFFFFFFu, upper ? t[2 * i] : t[2 * i + 1], 2);
+      if (pos >= valid) x = -INFINITY;
+      float mx = x;
       mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 4));
       mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 8));
       mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 16));
-      const float m_new = fmaxf(m[h], mx * scale_log2), base = m_new == -INFINITY ? 0.0f : m_new;
-      al[h] = ex2(m[h] - base);
-      s[h] = ex2(fmaf(s[h], scale_log2, -base));  // from here on the weight
-      l[h] = fmaf(l[h], al[h], s[h]);             // (of this lane's position: the lanes meet in finish())
-      m[h] = m_new;
+      const float m_new = fmaxf(m[i], mx * scale_log2), base = m_new == -INFINITY ? 0.0f : m_new;
+      al_own[i] = ex2(m[i] - base);
+      w_own[i] = ex2(fmaf(x, scale_log2, -base));
+      l[i] = fmaf(l[i], al_own[i], w_own[i]);  // (of this lane's position: the lanes meet in finish())
+      m[i] = m_new;
     }
-    // The weights [position][head] where the K rows were: every lane has read its part of them.
-    __syncwarp();
-    if (part == 0) {
-#pragma unroll
-      for (int h = 0; h < H; h += 4) *reinterpret_cast<float4 *>(stage + pos * 32u + 4 * h) = make_float4(s[h], s[h + 1], s[h + 2], s[h + 3]);
-    }
+    // The weights [position][head], and what the outputs so far count for, where the K rows were: every lane has read its part of them.
+    float *ws = reinterpret_cast<float *>(stage), *als = ws + Gm::CH * AP_HEADS;
     __syncwarp();
 #pragma unroll
-    for (int h = 0; h < H; h++)
+    for (int i = 0; i < H / 4; i++) {
+      ws[pos * AP_HEADS + 4 * i + part] = w_own[i];
+      if (pos == 0) als[4 * i + part] = al_own[i];
+    }
+    __syncwarp();
 #pragma unroll
-      for (int d = 0; d < DPL; d++) o[h][d] *= al[h];
+    for (int h = 0; h < H; h += 4) {
+      const float4 x = *reinterpret_cast<const float4 *>(als + h);
+#pragma unroll
+      for (int d = 0; d < DPL; d++) o[h][d] *= x.x, o[h + 1][d] *= x.y, o[h + 2][d] *= x.z, o[h + 3][d] *= x.w;
+    }
     const uint8_t *vs = stage + Gm::CH * Gm::ROWB;
 #pragma unroll
     for (int j = 0; j < Gm::CH; j++) {
@@ -316,14 +325,16 @@ struct ApWarp<float, HD, W> {
   }
   __device__ __forceinline__ void finish(float *red, float *ml, int lane) {
 #pragma unroll
-    for (int h = 0; h < AP_HEADS; h++) {
-      float sum = l[h];
+    for (int h = 0; h < AP_HEADS; h++)
+#pragma unroll
+      for (int d = 0; d < DPL; d++) red[Gm::red_at(h, lane * DPL + d)] = o[h][d];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      float sum = l[i];
       sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 4);
       sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 8);
       sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 16);
-#pragma unroll
-      for (int d = 0; d < DPL; d++) red[Gm::red_at(h, lane * DPL + d)] = o[h][d];
-      if (lane == 0) ml[2 * h] = m[h], ml[2 * h + 1] = sum;
+      if (lane < 4) ml[2 * (4 * i + lane)] = m[i], ml[2 * (4 * i + lane) + 1] = sum;
     }
   }
 };
