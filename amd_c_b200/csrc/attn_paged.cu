@@ -692,12 +692,13 @@ static int launch_ap(PagedAttnArgs &a, cudaStream_t st) {
   return IE_B200_OK;
 }
 // Eight warps to a CTA, or four and twice the CTAs: eight where there are few units, whose parts are then longer and fewer to merge (1 x
-// 32768 positions of 8 KV heads 30.3 against 34.0 us, of 4 22.3 / 28.6; at 64 units, 8 x 1000, 14.5 / 14.2), and where they may be
-// long (64 x 8192 at most 92.0 / 93.8); four where a unit's end comes often (32 x 1000 29.6 / 27.6, 256 x 200 64 / 51) and, for its
-// arithmetic, with the float cache (64 x 3001 at most 158 / 145). What the host knows of the lengths is how wide the table is.
+// 32768 positions of 8 KV heads 28.8 against 30.4 us, 1 x 4000 11.6 / 12.4; at 64 units, 8 x 8192 at most, 33.7 / 32.3), and with the half
+// cache where units have many heads and may be long (28 x 4 heads: 64 x 8192 at most 90.1 / 91.6, 32 x 4096 29.7 / 31.8; with 32 x 8
+// 172 / 168, 128 x 2500 at most 108 / 101). Four else: a unit's end waits for fewer warps (256 x 200 57 / 45; float cache, 64 x 3001 at most, 137 / 132).
+// What the host knows of the lengths is how wide the table is.
 template <typename KV, int HD>
 static int launch_ap(PagedAttnArgs &a, cudaStream_t st) {
-  const bool few = 2u * (uint64_t)a.R * a.kv.n_kv * a.groups <= (uint32_t)sm_count(), maybe_long = sizeof(KV) == 2 && table_positions(a.kv) >= 2048u;
+  const bool few = 4u * (uint64_t)a.R * a.kv.n_kv * a.groups <= (uint32_t)sm_count(), maybe_long = sizeof(KV) == 2 && a.gw > 4u && table_positions(a.kv) >= 2048u;
   return few || maybe_long ? launch_ap<KV, HD, 8>(a, st) : launch_ap<KV, HD, 4>(a, st);
 }
 
