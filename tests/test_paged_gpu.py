@@ -243,6 +243,30 @@ def test_attn_decode_paged_pages_that_do_not_exist(cuda, dtype):
     check_attention(out, None, *attention(q[2:], kp, vp, whole[2:3], [64], 4))
 
 
+@pytest.mark.parametrize("dtype", [torch.half, torch.float])
+@pytest.mark.parametrize("hd,rows,page", [(32, 1, 16), (32, 30, 48), (64, 1, 32), (64, 30, 16), (128, 1, 16), (128, 30, 80)])
+def test_attn_decode_paged_holes(cuda, dtype, hd, rows, page):
+    """Every third page of a sequence is none, first, last and neighbouring ones among them; what is left is attended to, few and many rows."""
+    lens = [900 + 37 * i % 700 for i in range(rows)]
+    q, kp, vp, table, n = case(hd + rows, lens, 8, 2, hd, page, dtype)
+    gen = torch.Generator().manual_seed(rows)
+    hole = (torch.rand(table.shape, generator=gen) < 0.34).to(cuda)
+    hole[0, 0] = hole[0, (lens[0] - 1) // page] = True
+    holes = torch.where(hole, -1 - torch.randint(0, 9, table.shape, generator=gen).int().to(cuda), table)
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    out, oq = K.attn_decode_paged(q, kp, vp, holes, n, 8, K.PagedScratch(8, 2, hd, cuda), err=err)
+    assert int(err) == PAGES_WORD
+    want, bound = torch.zeros(rows, 8, hd, dtype=torch.float64, device=cuda), torch.zeros(rows, 8, 1, dtype=torch.float64, device=cuda)
+    for r, m in enumerate(lens):
+        there = ~hole[r].repeat_interleave(page)[:m]
+        k, v = (get(p, table, r, m)[there].double().repeat_interleave(4, 1) for p in (kp, vp))
+        x = torch.einsum("hd,nhd->hn", q[r].double().view(8, hd), k) / hd ** 0.5
+        want[r] = torch.einsum("hn,nhd->hd", torch.softmax(x, 1), v)
+        size = torch.einsum("hd,nhd->hn", q[r].double().abs().view(8, hd), k.abs()) / hd ** 0.5
+        bound[r] = ((size.amax(1) + 1) * v.abs().amax((0, 2)))[:, None]
+    check_attention(out, oq, want, bound)
+
+
 def test_attn_decode_paged_many_rows_most_of_them_empty(cuda):
     """More rows than the GPU has warps: rows of nothing are zeros wherever they lie, padding keeps what it had."""
     q, kp, vp, table, _ = case(12, [33, 70], 4, 2, 64, 16, torch.half)
