@@ -380,7 +380,7 @@ def rope_kv_paged(qkv: torch.Tensor, kp: torch.Tensor, vp: torch.Tensor, table: 
         _refuse("cos", cos, _F32, (None, half), dev, "contiguous")
     s, p, q = _flat("sin", sin, _F32, (n_rope, half), dev), _flat("pos", pos, _I32, (T,), dev), _seq(seq, T, n_seq, dev)
     if out is None:
-        out, out_step = torch.empty_strided((T, nq * hd), (nq * hd, 1), dtype=_F32, device=qkv.device), nq * hd  # (half the time of torch.empty)
+        out, out_step = qkv.new_empty_strided((T, nq * hd), (nq * hd, 1)), nq * hd  # (two thirds of the time of torch.empty)
         to = out.data_ptr()
     else:
         to, _, _, out_step = _rows("out", out, _F32, T, nq * hd, dev)
@@ -394,7 +394,7 @@ class PagedScratch:
 
     def __init__(self, n_head: int, n_kv: int, hd: int, device):
         self.data = torch.zeros(_lib.load().ie_b200_attn_decode_paged_scratch_bytes(n_head, n_kv, hd), dtype=torch.uint8, device=device)
-        self.layout = (n_head, n_kv, hd)
+        self.layout, self.at, self.dev = (n_head, n_kv, hd), self.data.data_ptr(), self.data.get_device()
 
 
 def attn_decode_paged(q: torch.Tensor, kp: torch.Tensor, vp: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, n_head: int, scratch: PagedScratch,
@@ -404,16 +404,16 @@ def attn_decode_paged(q: torch.Tensor, kp: torch.Tensor, vp: torch.Tensor, table
     more (-1 too) is left as it was."""
     pages, dev, n_kv, hd, n_seq = _kv_pages(kp, vp, table)
     at, R, _, step = _rows("q", q, _F32, None, n_head * hd, dev)
-    if scratch.layout != (n_head, n_kv, hd) or scratch.data.get_device() != dev:
+    if scratch.layout != (n_head, n_kv, hd) or scratch.dev != dev:
         raise ValueError(f"scratch for {scratch.layout} (heads, KV heads, head size) on {scratch.data.device}, not {(n_head, n_kv, hd)} on cuda:{dev}")
     n, sq, row, nbq = _flat("lens", lens, _I32, (R,), dev), _seq(seq, R, n_seq, dev), n_head * hd, n_head * hd // 32
     if out is None:
-        out, out_step = torch.empty_strided((R, row), (row, 1), dtype=_F32, device=q.device), row
+        out, out_step = torch.empty_like(q) if step == row else q.new_empty_strided((R, row), (row, 1)), row
         to = out.data_ptr()
     else:
         to, _, _, out_step = _rows("out", out, _F32, R, row, dev)
     oq = torch.empty((R, q8_bytes(nbq)), dtype=torch.uint8, device=q.device) if quant else None
-    _run(_lib.load().ie_b200_attn_decode_paged, dev, (at, pages, to, _p(oq), n, sq, n_head, R, step * 4, out_step * 4, q8_bytes(nbq), scratch.data.data_ptr(),
+    _run(_lib.load().ie_b200_attn_decode_paged, dev, (at, pages, to, _p(oq), n, sq, n_head, R, step * 4, out_step * 4, q8_bytes(nbq), scratch.at,
                                                       None if err is None else _flat("err", err, _I32, (1,), dev)))
     return out, oq
 
@@ -428,8 +428,9 @@ def sample(x: torch.Tensor, u: torch.Tensor, temp: torch.Tensor | None = None, t
     dev = x.get_device()
     at, T, n, step = _rows("x", x, _F32, None, None, dev)
     row = (T,)
-    idx, prob = (torch.empty_strided(row, (1,), dtype=dt, device=x.device) for dt in (_I32, _F32))
-    _run(_lib.load().ie_b200_sample, dev, (at, n, idx.data_ptr(), prob.data_ptr(), _flat("u", u, _F32, row, dev),
+    uniform = _flat("u", u, _F32, row, dev)
+    idx, prob = torch.empty_strided(row, (1,), dtype=_I32, device=x.device), torch.empty_like(u)
+    _run(_lib.load().ie_b200_sample, dev, (at, n, idx.data_ptr(), prob.data_ptr(), uniform,
                                            None if temp is None else _flat("temp", temp, _F32, row, dev), None if top_k is None else _flat("top_k", top_k, _I32, row, dev),
                                            None if top_p is None else _flat("top_p", top_p, _F32, row, dev),
                                            None if min_p is None else _flat("min_p", min_p, _F32, row, dev), T, step * 4))
