@@ -24,6 +24,7 @@
 // 128: 64 rows of up to 3001, 132 us = 6.3 TB/s; of 64: 253 rows of 868 141 us = 6.4 TB/s.
 #include <cuda_pipeline_primitives.h>
 #include <math.h>
+#include <type_traits>
 
 #include "paged.cuh"
 #include "row_store.cuh"
@@ -351,7 +352,8 @@ __device__ __forceinline__ uint32_t ap_row(const PagedAttnArgs &a, uint32_t r, u
   return seq < a.kv.n_seq ? min(__ldg(a.len + r), table_positions(a.kv)) : 0u;
 }
 
-template <typename KV, int HD, int W>
+// MANY: more units than CTAs (half cache).
+template <typename KV, int HD, int W, bool MANY>
 __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_kernel(const PagedAttnArgs a) {
   using Gm = ApGeom<KV, HD, W>;
   constexpr int WARPS = W, THREADS = 32 * W, STAGES = Gm::STAGES;
@@ -391,15 +393,24 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
   };
   // Behind the chunks of a unit come some numbers without any, for what its end costs (about as long as a chunk of each warp).
   constexpr uint32_t END = WARPS;
-  uint32_t before, mine = 0u;  // (chunk numbers fit in 32 bits: the launcher sees to it)
+  uint32_t longest = 0u, before = 0u, mine = 0u;  // (chunk numbers fit in 32 bits: the launcher sees to it)
   for (uint32_t r = r_lo; r < r_hi; r++) {
     const uint32_t lc = chunks(r);
-    mine += lc ? lc + END : 0u;
+    mine += lc ? lc + END : 0u, longest = max(longest, lc);
   }
   uint32_t all = block_sum(mine, before) * units, share = (all + gridDim.x - 1u) / gridDim.x;
+  // More units than CTAs, and short: a warp has a unit to itself, and no two of them ever meet (235 rows of one position, 40 x 8 heads, 20 -> 9.6 us;
+  // 32 x 8: 256 of 50 21 -> 17, 256 of 1 to 200 39 -> 30; with longer ones, or fewer, a unit is too long a chain for one warp: 1200 units of 250 40 against 35,
+  // 300 of 60 8.3 against 6.2).
+  bool each_alone = false;
+  if constexpr (MANY) {
+    constexpr uint32_t MEAN = 9u, LONGEST = 18u;  // chunks
+    each_alone = all <= (uint64_t)(MEAN + END) * units * a.R && !__syncthreads_or(longest > LONGEST);
+    if (each_alone) all = 0u;
+  }
   if (share < a.min_share) share = a.min_share;
   uint32_t whole_shares = 1u;  // more: unit lengths are rounded up to a multiple of this
-  if (a.R <= gridDim.x && a.R * units <= gridDim.x) {  // a warp tries a length
+  if (!MANY && a.R <= gridDim.x && a.R * units <= gridDim.x) {  // a warp tries a length
     const uint32_t s = share + 2u * warp;
     uint32_t parts = 0u;
     for (uint32_t r = lane; r < a.R; r += 32u) parts += (chunks(r) + s - 1u) / s;
@@ -428,9 +439,20 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
   }
   __syncthreads();
 
-  if (x0 < x1) {
+  auto work = [&](auto by_warp) {
+    constexpr bool alone = decltype(by_warp)::value;
+    const uint32_t total_warps = gridDim.x * WARPS, own_unit = blockIdx.x * WARPS + warp;  // (alone) the first unit of this warp
+    if (alone ? own_unit >= a.R * units : x0 >= x1) return;
     ApCursor c;  // what is worked on
-    {
+    auto stand = [&](ApCursor &k) {  // (alone) at unit k.first of all; k.left: units left to this warp
+      k.r = k.first / units, k.unit = k.first - k.r * units;
+      k.len = ap_row(a, k.r, k.seq);
+      k.j0 = 0u, k.j1 = (k.len + CH - 1u) / CH;
+    };
+    if constexpr (alone) {
+      c.first = own_unit, c.left = (a.R * units - 1u - own_unit) / total_warps;
+      stand(c);
+    } else {
       c.r = misc[16];
       c.len = ap_row(a, c.r, c.seq);
       const uint32_t lc = (c.len + CH - 1u) / CH, num = numbered(lc);
@@ -441,6 +463,10 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
       c.left = x1 - end, c.j1 = min(lc, end - c.first);
     }
     auto advance = [&](ApCursor &k) {  // to the next unit (k.left > 0: there is one)
+      if constexpr (alone) {
+        k.first += total_warps, k.left--, stand(k);
+        return;
+      }
       k.first = x1 - k.left;
       if (++k.unit == units) {
         k.unit = 0u;
@@ -452,14 +478,15 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
       k.left = x1 - end, k.j0 = 0u, k.j1 = min(lc, end - k.first);
     };
     bool any = true;
-    if (c.j0 >= c.j1) {  // the share starts behind the chunks of a unit
+    if (!alone && c.j0 >= c.j1) {  // the share starts behind the chunks of a unit
       any = c.left != 0u;
       if (any) advance(c);
     }
 
     // ---- the ring: this warp's chunks, in the order in which they are worked on, STAGES - 1 ahead
     ApCursor f = c;  // what is fetched: chunk fj, in page column f_col of the sequence's row of the table f_row, chunk f_off of the page
-    uint32_t fj = f.j0 + warp, f_num = 0u, f_stage = 0u, f_col = fj / a.cpp, f_off = fj - f_col * a.cpp;
+    const uint32_t lane_of = alone ? 0u : warp, step = alone ? 1u : (uint32_t)WARPS;  // of this warp's chunks in a unit: the first, and from one to the next
+    uint32_t fj = f.j0 + lane_of, f_num = 0u, f_stage = 0u, f_col = fj / a.cpp, f_off = fj - f_col * a.cpp;
     const uint32_t *f_row = nullptr;
     size_t f_head = 0u;  // byte offset of the KV head in a page
     auto enter = [&] { f_row = a.kv.table + (size_t)f.seq * a.kv.table_stride, f_head = (size_t)(f.unit / a.groups) * a.kv.page * Gm::ROWB; };
@@ -472,7 +499,7 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
         }
         advance(f);
         enter();
-        fj = warp, f_col = warp / a.cpp, f_off = warp - f_col * a.cpp;
+        fj = lane_of, f_col = lane_of / a.cpp, f_off = lane_of - f_col * a.cpp;
       }
       f_num = f_row[f_col];
     };
@@ -503,7 +530,7 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
           }
         }
         if (lane == 0) valid_of[f_stage] = valid;
-        fj += WARPS, f_col += a.step_col, f_off += a.step_off;
+        fj += step, f_col += alone ? a.cpp == 1u : a.step_col, f_off += alone ? a.cpp != 1u : a.step_off;
         if (f_off >= a.cpp) f_off -= a.cpp, f_col++;
         find();
       }
@@ -531,9 +558,9 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
       uint32_t h0;
       const uint32_t heads = heads_of(c, h0);
       w.start(heads, reinterpret_cast<float *>(smem_ap + Gm::Q_OFF), tid);
-      uint32_t j = c.j0 + warp;
+      uint32_t j = c.j0 + lane_of;
       if constexpr (Gm::PAIRS) {
-        for (; j + WARPS < c.j1; j += 2u * WARPS) {
+        for (; j + step < c.j1; j += 2u * step) {
           __pipeline_wait_prior(STAGES - 3);
           __syncwarp();
           const uint32_t second = stage + 1u == STAGES ? 0u : stage + 1u;
@@ -546,7 +573,7 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
           stage = second + 1u == STAGES ? 0u : second + 1u;
         }
       }
-      for (; j < c.j1; j += WARPS) {
+      for (; j < c.j1; j += step) {
         __pipeline_wait_prior(STAGES - 2);
         __syncwarp();
         const uint32_t valid = valid_of[stage];
@@ -558,6 +585,24 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
       ApCursor next = c;
       const bool go_on = c.left != 0u;
       if (go_on) advance(next), load_q(next);
+      if constexpr (alone) {
+        w.finish(red + warp * AP_HEADS * HD, ml + warp * AP_HEADS * 2, lane);
+        __syncwarp();
+        if (c.j1) {
+#pragma unroll 2
+          for (uint32_t i0 = 0; i0 < heads * (HD / 4u); i0 += 32u) {
+            const uint32_t i = i0 + lane, h = min(i / (HD / 4u), AP_HEADS - 1u), d = i % (HD / 4u) * 4u;
+            const float L = ml[warp * AP_HEADS * 2 + 2 * h + 1], inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;  // (a NaN stays one)
+            const float4 v = *reinterpret_cast<const float4 *>(red + warp * AP_HEADS * HD + Gm::red_at(h, d));
+            store_row4<HD>(a.out, a.out_stride, a.oq, a.oq_stride, a.wide, a.n_head * HD / 32u, c.r, h0 + h, d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv),
+                           i < heads * (HD / 4u));
+          }
+        }
+        if (!go_on) break;
+        c = next;
+        __syncwarp();
+        continue;
+      }
       if (!Gm::F16) __syncthreads();  // (q lies where the records go)
       w.finish(red + warp * AP_HEADS * HD, ml + warp * AP_HEADS * 2, lane);
       __syncthreads();
@@ -651,6 +696,12 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
       __syncthreads();  // everybody has read the records (and misc): the next unit's may be written
     }
     __pipeline_wait_prior(0);
+  };
+  if constexpr (MANY) {
+    if (each_alone) work(std::true_type());
+    else work(std::false_type());
+  } else {
+    work(std::false_type());
   }
 
   // ---- rows that see nothing: zeros (a lane looks at a row, its warp writes it)
@@ -677,13 +728,14 @@ static size_t ap_record_bytes(uint32_t hd) { return (size_t)AP_HEADS * (hd + 4u)
 template <typename KV, int HD, int W>
 static int launch_ap(PagedAttnArgs &a, cudaStream_t st) {
   using Gm = ApGeom<KV, HD, W>;
-  auto k = attn_paged_kernel<KV, HD, W>;
-  if (int r = ensure_dynamic_smem(reinterpret_cast<const void *>(k), Gm::TOTAL)) return r;
   const uint32_t sms = (uint32_t)sm_count(), ctas = sms * Gm::CTAS < AP_MAX_CTAS ? sms * Gm::CTAS : AP_MAX_CTAS;
   a.cpp = a.kv.page / Gm::CH, a.step_col = W / a.cpp, a.step_off = W % a.cpp;
   a.min_share = 128u / Gm::CH;  // 128 positions: 1 x 100 of 8 KV heads in 5.5 us (64: 7.5, 256: 5.5), 1 x 500 in 8.1 (8.0, 9.3)
   for (uint32_t R = a.R; R;) {
     a.R = R < a.most ? R : a.most;
+    const uint64_t units = (uint64_t)a.R * a.kv.n_kv * a.groups;
+    const auto k = Gm::F16 && units > ctas && units < 1ull << 31 ? attn_paged_kernel<KV, HD, W, Gm::F16> : attn_paged_kernel<KV, HD, W, false>;
+    if (int r = ensure_dynamic_smem(reinterpret_cast<const void *>(k), Gm::TOTAL)) return r;
     IEB_LAUNCH_PDL("attn_paged_kernel", k, dim3(ctas), dim3(32 * W), Gm::TOTAL, st, a);
     R -= a.R;
     a.q = reinterpret_cast<const float *>(reinterpret_cast<const char *>(a.q) + a.q_stride * a.R), a.out = reinterpret_cast<float *>(reinterpret_cast<char *>(a.out) + a.out_stride * a.R);

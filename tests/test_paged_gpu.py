@@ -284,6 +284,40 @@ def test_attn_decode_paged_many_rows_most_of_them_empty(cuda):
     check_attention(out[full], oq[full], *attention(q[full], kp, vp, table, lens[full], 4, seq[full]))
 
 
+@pytest.mark.parametrize("dtype", [torch.half, torch.float])
+@pytest.mark.parametrize("n_head,n_kv,hd,page,extra", [(28, 4, 128, 16, 140), (40, 8, 128, 64, 1), (12, 1, 128, 48, 1), (16, 16, 64, 32, 1), (9, 1, 64, 16, 1), (8, 4, 32, 16, 1), (32, 2, 32, 80, 30)])
+def test_attn_decode_paged_many_short_rows(cuda, dtype, n_head, n_kv, hd, page, extra):
+    """More (row, KV head) pairs than the GPU has room for at once, of no to some chunks each; empty rows, padding, a missing page; narrow and wide tables."""
+    lens = [(i * 37) % 210 for i in range(41)]
+    gen = generator(hd + n_head)
+    kp, vp, table = make_cache(gen, lens, n_kv, hd, page, dtype, extra_cols=extra)
+    for s, n in enumerate(lens):
+        for pool in (kp, vp):
+            put(pool, table, s, torch.randn(n, n_kv, hd, device=cuda, generator=gen))
+    R = 1300
+    seq = (torch.arange(R, device=cuda, dtype=torch.int32) * 7) % 43 - 1  # -1 and 41 pad
+    real = (seq >= 0) & (seq < 41)
+    n = torch.tensor(lens, dtype=torch.int32, device=cuda)[seq.long().clamp(0, 40)]
+    n = (n - torch.arange(R, device=cuda, dtype=torch.int32) % 11).clamp(min=0)
+    q = torch.randn(R, n_head * hd, device=cuda, generator=gen)
+    out, scratch, err = torch.full_like(q, 4.0), K.PagedScratch(n_head, n_kv, hd, cuda), torch.zeros(1, dtype=torch.int32, device=cuda)
+    _, oq = K.attn_decode_paged(q, kp, vp, table, n, n_head, scratch, seq=seq, out=out, err=err)
+    assert int(err) == 0 and (out[~real] == 4).all()
+    assert (out[real & (n == 0)] == 0).all() and (oq[real & (n == 0)] == 0).all()
+    some = torch.nonzero(real)[:, 0]
+    check_attention(out[some], oq[some], *attention(q[some], kp, vp, table, n[some], n_head, seq[some]))
+    again, _ = K.attn_decode_paged(q, kp, vp, table, n, n_head, scratch, seq=seq, quant=False)
+    assert torch.equal(again[real], out[real])
+    table[5, 0] = -3  # sequence 5 has lost its first page
+    lost, _ = K.attn_decode_paged(q, kp, vp, table, n, n_head, scratch, seq=seq, quant=False, err=err)
+    assert int(err) == PAGES_WORD and torch.equal(lost[real & (seq != 5)], out[real & (seq != 5)])
+    mine = torch.nonzero((seq == 5) & (n > page))[:, 0]
+    if len(mine):
+        table[5, :-1] = table[5, 1:].clone()
+        check_attention(lost[mine], None, *attention(q[mine], kp, vp, table, n[mine] - page, n_head, seq[mine]))
+    assert (lost[(seq == 5) & (n <= page)] == 0).all()
+
+
 @pytest.mark.parametrize("own", [True, False])
 def test_attn_decode_paged_wide_tables(cuda, own):
     """Tables of 2^24 positions, of which little is in use: 300 rows are more than one launch numbers; rows of their own sequences, and rows that
