@@ -10,7 +10,8 @@
 // a unit (row, KV head, group) in turn; each warp has its own ring of buffers that it fills itself (cp.async, rows past the length
 // zero-filled) and its own running maximum, sum and outputs, so nothing in the stream waits for another warp, and the ring runs on into
 // the next unit while this one's records are merged. A unit that lies in one CTA is finished there; the parts of a cut one go to
-// global memory as (outputs, max, sum) records, and the CTA that finishes last adds them in the order of the positions.
+// global memory as (outputs, max, sum) records, and the CTA that finishes last adds them in the order of the positions. Where units are
+// many and short, each is one warp's instead, and nothing meets.
 //
 // Half cache: mma.sync m16n8k16, the positions on the 16-row side, the heads on the 8-column side (as attn_decode.cu). q and the
 // weights are carried as two f16 terms; every accumulation takes few MMAs (what the tensor cores cut off grows with their number) and is
@@ -232,10 +233,24 @@ struct ApWarp<float, HD, W> {
   }
   // (All threads call it, behind a barrier after which nobody reads what is at q_smem.)
   __device__ __forceinline__ void start(uint32_t heads, float *q_smem, uint32_t tid) {
-    few = heads <= 4u, qs = q_smem;
 #pragma unroll
     for (int i = 0; i < QPT; i++) q_smem[tid + 32u * W * i] = q[i];
     __syncthreads();
+    clear(heads, q_smem);
+  }
+  // The same for one warp, q from where it is.
+  __device__ __forceinline__ void start_alone(const float *src, uint32_t heads, float *q_smem, uint32_t lane) {
+#pragma unroll 8
+    for (uint32_t i = 4u * lane; i < heads * HD; i += 128u) {
+      const float2 a = *reinterpret_cast<const float2 *>(src + i), b = *reinterpret_cast<const float2 *>(src + i + 2);
+      *reinterpret_cast<float4 *>(q_smem + i) = make_float4(a.x, a.y, b.x, b.y);
+    }
+    for (uint32_t i = heads * HD + lane; i < AP_HEADS * HD; i += 32u) q_smem[i] = 0.0f;
+    __syncwarp();
+    clear(heads, q_smem);
+  }
+  __device__ __forceinline__ void clear(uint32_t heads, const float *q_smem) {
+    few = heads <= 4u, qs = q_smem;
 #pragma unroll
     for (int h = 0; h < AP_HEADS; h++)
 #pragma unroll
@@ -352,7 +367,7 @@ __device__ __forceinline__ uint32_t ap_row(const PagedAttnArgs &a, uint32_t r, u
   return seq < a.kv.n_seq ? min(__ldg(a.len + r), table_positions(a.kv)) : 0u;
 }
 
-// MANY: more units than CTAs (half cache).
+// MANY: more units than CTAs.
 template <typename KV, int HD, int W, bool MANY>
 __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_kernel(const PagedAttnArgs a) {
   using Gm = ApGeom<KV, HD, W>;
@@ -401,10 +416,10 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
   uint32_t all = block_sum(mine, before) * units, share = (all + gridDim.x - 1u) / gridDim.x;
   // More units than CTAs, and short: a warp has a unit to itself, and no two of them ever meet (235 rows of one position, 40 x 8 heads, 20 -> 9.6 us;
   // 32 x 8: 256 of 50 21 -> 17, 256 of 1 to 200 39 -> 30; with longer ones, or fewer, a unit is too long a chain for one warp: 1200 units of 250 40 against 35,
-  // 300 of 60 8.3 against 6.2).
+  // 300 of 60 8.3 against 6.2; float cache, 235 x 1 22 -> 13, 300 x 70 of 8 x 4 heads of 32 13.9 -> 11.7, 256 of 1 to 100, 32 x 8 of 64, 28 against 26).
   bool each_alone = false;
   if constexpr (MANY) {
-    constexpr uint32_t MEAN = 9u, LONGEST = 18u;  // chunks
+    constexpr uint32_t MEAN = 9u, LONGEST = Gm::F16 ? 18u : 9u;  // chunks
     each_alone = all <= (uint64_t)(MEAN + END) * units * a.R && !__syncthreads_or(longest > LONGEST);
     if (each_alone) all = 0u;
   }
@@ -547,17 +562,23 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
       h0 = kvh * a.G + grp * a.gw;
       return min(a.gw, a.G - grp * a.gw);
     };
+    auto q_of = [&](const ApCursor &k, uint32_t h0) { return reinterpret_cast<const float *>(reinterpret_cast<const char *>(a.q) + a.q_stride * k.r) + (size_t)h0 * HD; };
     auto load_q = [&](const ApCursor &k) {
       uint32_t h0;
       const uint32_t heads = heads_of(k, h0);
-      w.load(reinterpret_cast<const float *>(reinterpret_cast<const char *>(a.q) + a.q_stride * k.r) + (size_t)h0 * HD, heads, tid);
+      if (Gm::F16 || !alone) w.load(q_of(k, h0), heads, tid);
     };
     if (any) load_q(c);
     uint32_t stage = 0u;
     while (any) {
       uint32_t h0;
       const uint32_t heads = heads_of(c, h0);
-      w.start(heads, reinterpret_cast<float *>(smem_ap + Gm::Q_OFF), tid);
+      if constexpr (Gm::F16) {
+        w.start(heads, nullptr, tid);
+      } else {
+        if (alone) w.start_alone(q_of(c, h0), heads, red + warp * AP_HEADS * HD, lane);  // (where its record goes)
+        else w.start(heads, reinterpret_cast<float *>(smem_ap + Gm::Q_OFF), tid);
+      }
       uint32_t j = c.j0 + lane_of;
       if constexpr (Gm::PAIRS) {
         for (; j + step < c.j1; j += 2u * step) {
@@ -586,6 +607,7 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
       const bool go_on = c.left != 0u;
       if (go_on) advance(next), load_q(next);
       if constexpr (alone) {
+        __syncwarp();
         w.finish(red + warp * AP_HEADS * HD, ml + warp * AP_HEADS * 2, lane);
         __syncwarp();
         if (c.j1) {
@@ -734,7 +756,8 @@ static int launch_ap(PagedAttnArgs &a, cudaStream_t st) {
   for (uint32_t R = a.R; R;) {
     a.R = R < a.most ? R : a.most;
     const uint64_t units = (uint64_t)a.R * a.kv.n_kv * a.groups;
-    const auto k = Gm::F16 && units > ctas && units < 1ull << 31 ? attn_paged_kernel<KV, HD, W, Gm::F16> : attn_paged_kernel<KV, HD, W, false>;
+    constexpr bool CAN = Gm::F16 || W == 4;  // (eight warps with the float cache: few units)
+    const auto k = units > ctas && units < 1ull << 31 ? attn_paged_kernel<KV, HD, W, CAN> : attn_paged_kernel<KV, HD, W, false>;
     if (int r = ensure_dynamic_smem(reinterpret_cast<const void *>(k), Gm::TOTAL)) return r;
     IEB_LAUNCH_PDL("attn_paged_kernel", k, dim3(ctas), dim3(32 * W), Gm::TOTAL, st, a);
     R -= a.R;
