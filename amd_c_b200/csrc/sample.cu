@@ -301,14 +301,20 @@ struct Sampler {
   template <typename G>
   __device__ __forceinline__ void border(G goal_of) {
     cluster_sync_all();
-    for (uint32_t b = rank * (SM_BINS / cl) + tid; b < (rank + 1u) * (SM_BINS / cl); b += SM_THREADS) {  // this CTA's share of the bins, for all
-      uint32_t lo[SM_MAX_CL], hi[SM_MAX_CL];
+    const uint32_t side = tid & 1u;
+    for (uint32_t i = tid; i < 2u * (SM_BINS / cl); i += SM_THREADS) {  // this CTA's share of the bins, for all; two threads to a bin (whole warps: cl is at most 8)
+      const uint32_t b = rank * (SM_BINS / cl) + i / 2u;
+      uint32_t lo[SM_MAX_CL / 2], hi[SM_MAX_CL / 2];
 #pragma unroll
-      for (uint32_t c = 0; c < SM_MAX_CL; c++) lo[c] = c < cl ? dsm_ld32(peer(&s.low[b], c)) : 0u, hi[c] = c < cl ? dsm_ld32(peer(&s.high[b], c)) : 0u;
+      for (uint32_t c = 0; c < SM_MAX_CL / 2; c++) {
+        const uint32_t from = 2u * c + side;
+        lo[c] = from < cl ? dsm_ld32(peer(&s.low[b], from)) : 0u, hi[c] = from < cl ? dsm_ld32(peer(&s.high[b], from)) : 0u;
+      }
       uint64_t v = 0u;
 #pragma unroll
-      for (uint32_t c = 0; c < SM_MAX_CL; c++) v += (uint64_t)hi[c] << 32 | lo[c];
-      for (uint32_t c = 0; c < cl; c++) dsm_st64(peer(&s.bins[b], c), v);
+      for (uint32_t c = 0; c < SM_MAX_CL / 2; c++) v += (uint64_t)hi[c] << 32 | lo[c];
+      v += __shfl_xor_sync(0xFFFFFFFFu, v, 1);
+      for (uint32_t c = side; c < cl; c += 2u) dsm_st64(peer(&s.bins[b], c), v);
     }
     cluster_sync_all();
     const uint64_t v[SM_PER] = {s.bins[SM_PER * tid], s.bins[SM_PER * tid + 1u], s.bins[SM_PER * tid + 2u]};
