@@ -763,12 +763,18 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(const SampleArgs 
                  [&](uint32_t idx, uint64_t w, uint64_t all) { sample_out(a, row, idx, (float)((double)w / (double)all)); });
 }
 
-// CTAs of a row: as many as leave each 2000 logits, while the batch stays within two rounds of what runs at once (1 x 32003, all kinds mixed: 1 CTA
-// 13.6 us, 4 8.5, 8 7.6; 37 rows 36 / 19 / 17; 128 rows 37 / 27 / 40; 37 x 16000 20 / 13 / 13; 32 x 4000 11.5 / 9.3 / 11.6), and as many as
-// the slices need.
+// CTAs of a row: as many as leave each 2000 logits while the batch runs at once (clusters lie within a part of the GPU each, so that is about
+// 7/4 of the SMs, not twice), 4000 up to two rounds of it, and as many as the slices need. 1 x 32003, all kinds mixed: 1 CTA 13.6 us, 4 8.5,
+// 8 7.2; 28 rows 4 18.9, 8 15.7; 37 rows 4 19, 8 17 (of one kind, top-k 50, 11 and 13.5); 128 rows 1 37, 4 27, 8 40; 64 x 16000 4 14.8, 8 19.2;
+// 64 x 100000 38 and 30; 32 x 4000 1 11.5, 4 9.3, 8 11.6.
 static uint32_t sample_ctas(uint32_t n, uint32_t T) {
+  const uint64_t sms = (uint64_t)sm_count();
   uint32_t c = 1u;
-  while (c < (uint32_t)SM_MAX_CL && (n > c * SM_MAX_SLICE || (n >= 4000u * c && (uint64_t)T * c * 2u <= 4u * (uint32_t)sm_count()))) c *= 2u;
+  auto more = [&] {  // twice as many?
+    const uint64_t ctas = (uint64_t)T * c * 2u;
+    return n > c * SM_MAX_SLICE || (ctas <= 4u * sms && n >= (4u * ctas <= 7u * sms ? 4000u : 8000u) * c);
+  };
+  while (c < (uint32_t)SM_MAX_CL && more()) c *= 2u;
   return c;
 }
 
