@@ -43,6 +43,7 @@ SIGNATURES = {
     "ie_b200_gemv_norm_tail": (_int, [_int, _vp, _u32, _u32, _vp, _vp, _vp, _vp, _vp, _f32, _vp, _vp, _vp, _vp]),
     "ie_b200_block_dots": (_int, [_int, _vp, _u32, _u32, _vp, _vp, _vp]),
     "ie_b200_embed": (_int, [_int, _vp, _u32, _vp, _vp, _u32, _sz, _vp]),
+    "ie_b200_embed_rows": (_int, [_int, _vp, _u32, _u32, _vp, _vp, _u32, _sz, _vp]),
     "ie_b200_rmsnorm": (_int, [_vp, _vp, _vp, _u32, _f32, _vp, _u32, _sz, _sz, _sz, _vp]),
     "ie_b200_swiglu": (_int, [_vp, _vp, _u32, _vp, _u32, _sz, _sz, _vp]),
     "ie_b200_swiglu_il": (_int, [_vp, _vp, _u32, _vp, _u32, _sz, _sz, _sz, _vp]),

@@ -29,11 +29,18 @@ __global__ void __launch_bounds__(256) quant_q8_kernel(const float *x, uint8_t *
 }
 
 // ---- embedding row ----
-__global__ void __launch_bounds__(256) embed_q4_kernel(const uint8_t *w, size_t rowb, uint32_t nb, const uint32_t *tok, float *out, size_t os) {
+// A token that the matrix has no row for: zeros. True where that was so.
+__device__ __forceinline__ bool embed_nothing(uint32_t id, uint32_t rows, uint32_t cols, float *o) {
+  if (id < rows) return false;
+  for (uint32_t e = blockIdx.x * blockDim.x + threadIdx.x; e < cols; e += gridDim.x * blockDim.x) o[e] = 0.0f;
+  return true;
+}
+__global__ void __launch_bounds__(256) embed_q4_kernel(const uint8_t *w, size_t rowb, uint32_t rows, uint32_t nb, const uint32_t *tok, float *out, size_t os) {
   pdl_prologue();
-  const uint32_t t = blockIdx.y;
-  const uint8_t *rp = w + (size_t)tok[t] * rowb;
+  const uint32_t t = blockIdx.y, id = tok[t];
+  const uint8_t *rp = w + (size_t)id * rowb;
   float *o = row_ptr(out, os, t);
+  if (embed_nothing(id, rows, nb * 32u, o)) return;
   for (uint32_t e = blockIdx.x * blockDim.x + threadIdx.x; e < nb * 32u; e += gridDim.x * blockDim.x) {
     const uint32_t b = e >> 5, j = e & 31u;
     const uint32_t word = reinterpret_cast<const uint32_t *>(rp + 16u * (size_t)b)[(j & 15u) >> 2];
@@ -43,21 +50,23 @@ __global__ void __launch_bounds__(256) embed_q4_kernel(const uint8_t *w, size_t 
   }
 }
 // Q8_0 row: d * (float)(int8) weight (mat_row, src/cpu.c:257-265)
-__global__ void __launch_bounds__(256) embed_q8_kernel(const uint8_t *w, size_t rowb, uint32_t nb, const uint32_t *tok, float *out, size_t os) {
+__global__ void __launch_bounds__(256) embed_q8_kernel(const uint8_t *w, size_t rowb, uint32_t rows, uint32_t nb, const uint32_t *tok, float *out, size_t os) {
   pdl_prologue();
-  const uint32_t t = blockIdx.y;
-  const uint8_t *rp = w + (size_t)tok[t] * rowb;
+  const uint32_t t = blockIdx.y, id = tok[t];
+  const uint8_t *rp = w + (size_t)id * rowb;
   float *o = row_ptr(out, os, t);
+  if (embed_nothing(id, rows, nb * 32u, o)) return;
   for (uint32_t e = blockIdx.x * blockDim.x + threadIdx.x; e < nb * 32u; e += gridDim.x * blockDim.x) {
     const float d = h2f(reinterpret_cast<const uint16_t *>(rp + 32u * (size_t)nb)[e >> 5]);
     o[e] = __fmul_rn(d, (float)reinterpret_cast<const int8_t *>(rp)[e]);
   }
 }
-__global__ void __launch_bounds__(256) embed_f32_kernel(const float *w, uint32_t cols, const uint32_t *tok, float *out, size_t os) {
+__global__ void __launch_bounds__(256) embed_f32_kernel(const float *w, uint32_t rows, uint32_t cols, const uint32_t *tok, float *out, size_t os) {
   pdl_prologue();
-  const uint32_t t = blockIdx.y;
-  const float *rp = w + (size_t)tok[t] * cols;
+  const uint32_t t = blockIdx.y, id = tok[t];
+  const float *rp = w + (size_t)id * cols;
   float *o = row_ptr(out, os, t);
+  if (embed_nothing(id, rows, cols, o)) return;
   for (uint32_t e = blockIdx.x * blockDim.x + threadIdx.x; e < cols; e += gridDim.x * blockDim.x) o[e] = rp[e];
 }
 
@@ -405,27 +414,37 @@ extern "C" int ie_b200_quant_q8(const float *d_x, void *d_q, uint32_t nb, uint32
   return IE_B200_OK;
 }
 
-extern "C" int ie_b200_embed(int kind, const void *d_w, uint32_t cols, const uint32_t *d_tok, float *d_out, uint32_t T, size_t out_stride,
-                             void *stream) {
-  if (!d_w || !d_tok || !d_out) return fail(IE_B200_E_ARG, "ie_b200_embed: NULL pointer");
+static int embed_of(const char *who, int kind, const void *d_w, uint32_t rows, uint32_t cols, const uint32_t *d_tok, float *d_out, uint32_t T, size_t out_stride,
+                    void *stream) {
+  if (!d_w || !d_tok || !d_out) return fail(IE_B200_E_ARG, "%s: NULL pointer", who);
   if (T == 0 || cols == 0) return IE_B200_OK;
-  if (T > 65535u) return fail(IE_B200_E_SIZE, "ie_b200_embed: T %u > 65535", T);
+  if (T > 65535u) return fail(IE_B200_E_SIZE, "%s: T %u > 65535", who, T);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const dim3 grid((cols + 255u) / 256u, T);
   if (kind == IE_B200_MAT_Q4) {
-    if (cols % 32u) return fail(IE_B200_E_SIZE, "ie_b200_embed: cols %u is not a multiple of 32", cols);
-    IEB_LAUNCH_PDL("embed_q4_kernel", embed_q4_kernel, grid, dim3(256), 0, st, static_cast<const uint8_t *>(d_w), row_bytes_of(kind, cols),
+    if (cols % 32u) return fail(IE_B200_E_SIZE, "%s: cols %u is not a multiple of 32", who, cols);
+    IEB_LAUNCH_PDL("embed_q4_kernel", embed_q4_kernel, grid, dim3(256), 0, st, static_cast<const uint8_t *>(d_w), row_bytes_of(kind, cols), rows,
                    cols / 32u, d_tok, d_out, out_stride);
   } else if (kind == IE_B200_MAT_Q8) {
-    if (cols % 32u) return fail(IE_B200_E_SIZE, "ie_b200_embed: cols %u is not a multiple of 32", cols);
-    IEB_LAUNCH_PDL("embed_q8_kernel", embed_q8_kernel, grid, dim3(256), 0, st, static_cast<const uint8_t *>(d_w), row_bytes_of(kind, cols),
+    if (cols % 32u) return fail(IE_B200_E_SIZE, "%s: cols %u is not a multiple of 32", who, cols);
+    IEB_LAUNCH_PDL("embed_q8_kernel", embed_q8_kernel, grid, dim3(256), 0, st, static_cast<const uint8_t *>(d_w), row_bytes_of(kind, cols), rows,
                    cols / 32u, d_tok, d_out, out_stride);
   } else if (kind == IE_B200_MAT_F32) {
-    IEB_LAUNCH_PDL("embed_f32_kernel", embed_f32_kernel, grid, dim3(256), 0, st, static_cast<const float *>(d_w), cols, d_tok, d_out, out_stride);
+    IEB_LAUNCH_PDL("embed_f32_kernel", embed_f32_kernel, grid, dim3(256), 0, st, static_cast<const float *>(d_w), rows, cols, d_tok, d_out, out_stride);
   } else {
-    return fail(IE_B200_E_ARG, "ie_b200_embed: kind %d has no embedding kernel", kind);
+    return fail(IE_B200_E_ARG, "%s: kind %d has no embedding kernel", who, kind);
   }
   return IE_B200_OK;
+}
+
+extern "C" int ie_b200_embed(int kind, const void *d_w, uint32_t cols, const uint32_t *d_tok, float *d_out, uint32_t T, size_t out_stride,
+                             void *stream) {
+  return embed_of("ie_b200_embed", kind, d_w, 0xFFFFFFFFu, cols, d_tok, d_out, T, out_stride, stream);
+}
+
+extern "C" int ie_b200_embed_rows(int kind, const void *d_w, uint32_t rows, uint32_t cols, const uint32_t *d_tok, float *d_out, uint32_t T,
+                                  size_t out_stride, void *stream) {
+  return embed_of("ie_b200_embed_rows", kind, d_w, rows, cols, d_tok, d_out, T, out_stride, stream);
 }
 
 extern "C" int ie_b200_rmsnorm(const float *d_x, const float *d_w, float *d_y, uint32_t n, float eps, void *d_q, uint32_t T, size_t x_stride,

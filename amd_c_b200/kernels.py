@@ -159,9 +159,10 @@ def block_dots(w: Mat, xq: torch.Tensor) -> torch.Tensor:
 
 
 def embed(w: Mat, tok: torch.Tensor) -> torch.Tensor:
+    """Rows tok [T] int32 of w; a token that is no row of it (a draw's -1 too) gives zeros."""
     T = tok.numel()
     out = torch.empty((T, w.cols), dtype=torch.float32, device=tok.device)
-    check(_lib.load().ie_b200_embed(w.kind, w.data.data_ptr(), w.cols, tok.data_ptr(), out.data_ptr(), T, w.cols * 4, _stream()))
+    check(_lib.load().ie_b200_embed_rows(w.kind, w.data.data_ptr(), w.rows, w.cols, tok.data_ptr(), out.data_ptr(), T, w.cols * 4, _stream()))
     return out
 
 

@@ -165,9 +165,13 @@ int ie_b200_block_dots(int kind, const void *d_w, uint32_t rows, uint32_t cols, 
 
 /* Row `tok` of the token embedding as floats (MAT_Q4, MAT_Q8 or MAT_F32):
  * mat_row (src/cpu.c:252-274), ie_embed_q4 / _f32 (kernels/ie_kernels.c:171-191).
- * d_tok: T token ids on the device. */
+ * d_tok: T token ids on the device, each of them a row of the matrix (nothing checks that; 0xFFFFFFFF alone gives zeros). */
 int ie_b200_embed(int kind, const void *d_w, uint32_t cols, const uint32_t *d_tok, float *d_out, uint32_t T, size_t out_stride,
                   void *stream);
+/* The same for tokens that come from the device, from ie_b200_sample or ie_b200_argmax: a token of `rows` (of the matrix) or more, such
+ * as the 0xFFFFFFFF of a row with nothing to draw or of one that pads a batch, gives a row of zeros. */
+int ie_b200_embed_rows(int kind, const void *d_w, uint32_t rows, uint32_t cols, const uint32_t *d_tok, float *d_out, uint32_t T,
+                       size_t out_stride, void *stream);
 
 /* y = x * rsqrt(mean x^2 + eps) * w, optionally with the Q8 copy of y
  * (d_q != NULL): rmsnorm (src/cpu.c:276-281) + cpu_quant_q8; ie_rmsnorm
@@ -316,7 +320,8 @@ int ie_b200_topk(const float *d_x, uint32_t nv, uint32_t K, uint32_t T, size_t x
  * counts as 0, 1 and more as just below 1); the probability is w_i over that sum. temp 0 (or less, or NaN): the first maximum,
  * probability 1; a temp below 2^-126 counts as that. Weights are integers of 2^-44 of the largest one (2^-43 above 2^18 tokens; finer
  * for shorter rows), their sums exact; a token whose weight rounds to 0 is not drawn. A NaN logit is never drawn, one of -inf neither,
- * nor one that is further from the maximum than a float reaches; a row with nothing else gives index 0xFFFFFFFF and probability 0; where
+ * nor one that is further from the maximum than a float reaches; a row with nothing else gives index 0xFFFFFFFF and probability 0 (a token
+ * that only ie_b200_embed_rows takes); where
  * the maximum is +inf its tokens are equally likely. d_u: T uniform numbers in [0, 1). d_temp, d_top_k, d_top_p, d_min_p: T values
  * each, or NULL (1, 0, 1, 0). n up to 360448, T up to 2^20. No scratch. The role of the reference's host sampler behind
  * backend.topk (src/gen.c, src/backend.h:33-37), which knows temp and top_k. */
