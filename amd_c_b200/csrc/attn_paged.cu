@@ -43,7 +43,7 @@ struct PagedAttnArgs {
   uint32_t *count, *err;
   ie_b200_kv_pages kv;
   uint32_t n_head, G, groups, gw, R, wide, seq0;  // groups: head groups of a KV head, gw heads each (the last may have fewer); seq0: sequence of row 0 where seq is NULL
-  uint32_t min_share, most;  // most: rows of a launch
+  uint32_t min_share, most, fill;  // most: rows of a launch; fill: outputs whose rows of padding are zeros (1: out, 2: oq)
   uint32_t cpp, step_col, step_off;  // chunks of a page; a warp's step from chunk to chunk, in pages and chunks
   size_t q_stride, out_stride, oq_stride;
   float scale_log2;  // log2(e) / sqrt(hd)
@@ -726,7 +726,7 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
     work(std::false_type());
   }
 
-  // ---- rows that see nothing: zeros (a lane looks at a row, its warp writes it)
+  // ---- rows that see nothing, and the padding of new outputs: zeros (a lane looks at a row, its warp writes it)
   const uint32_t warps = gridDim.x * WARPS;
   for (uint32_t r0 = blockIdx.x * WARPS + warp; r0 < a.R; r0 += 32u * warps) {
     const uint32_t r = r0 + lane * warps;
@@ -734,11 +734,13 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
     if (r < a.R) len = ap_row(a, r, seq);
     const bool real = r < a.R && seq < a.kv.n_seq;
     if (real && a.err && __ldg(a.len + r) > len) atomicExch(a.err, ERR_PAGES);
-    for (uint32_t empty = __ballot_sync(0xFFFFFFFFu, real && len == 0u); empty; empty &= empty - 1u) {
-      const uint32_t e = r0 + (__ffs(empty) - 1u) * warps;
+    const uint32_t reals = __ballot_sync(0xFFFFFFFFu, real);
+    for (uint32_t empty = __ballot_sync(0xFFFFFFFFu, r < a.R && len == 0u && (real || a.fill)); empty; empty &= empty - 1u) {
+      const uint32_t k = __ffs(empty) - 1u, e = r0 + k * warps, which = reals >> k & 1u ? 3u : a.fill;
       float *out = reinterpret_cast<float *>(reinterpret_cast<char *>(a.out) + a.out_stride * e);
-      for (uint32_t i = lane; i < a.n_head * HD; i += 32u) out[i] = 0.0f;
-      if (a.oq)
+      if (which & 1u)
+        for (uint32_t i = lane; i < a.n_head * HD; i += 32u) out[i] = 0.0f;
+      if (a.oq && (which & 2u))
         for (uint32_t i = lane; i < a.n_head * HD / 32u * 10u; i += 32u) reinterpret_cast<uint32_t *>(a.oq + a.oq_stride * e)[i] = 0u;
     }
   }
@@ -789,11 +791,18 @@ extern "C" size_t ie_b200_attn_decode_paged_scratch_bytes(uint32_t n_head, uint3
 extern "C" int ie_b200_attn_decode_paged(const float *d_q, const ie_b200_kv_pages *pages, float *d_out, void *d_oq, const uint32_t *d_len, const uint32_t *d_seq,
                                          uint32_t n_head, uint32_t R, size_t q_stride, size_t out_stride, size_t oq_stride, void *d_scratch, uint32_t *d_err,
                                          void *stream) {
+  return ie_b200_attn_decode_paged_fill(d_q, pages, d_out, d_oq, d_len, d_seq, n_head, R, q_stride, out_stride, oq_stride, d_scratch, d_err, 0u, stream);
+}
+
+extern "C" int ie_b200_attn_decode_paged_fill(const float *d_q, const ie_b200_kv_pages *pages, float *d_out, void *d_oq, const uint32_t *d_len, const uint32_t *d_seq,
+                                              uint32_t n_head, uint32_t R, size_t q_stride, size_t out_stride, size_t oq_stride, void *d_scratch, uint32_t *d_err,
+                                              uint32_t fill, void *stream) {
   if (R == 0) return IE_B200_OK;  // (an empty tensor may have no address)
   if (int r = check_pages("ie_b200_attn_decode_paged", pages, 16u)) return r;
   if (!d_q || !d_out || !d_len || !d_scratch) return fail(IE_B200_E_ARG, "ie_b200_attn_decode_paged: NULL pointer");
   if ((((uintptr_t)d_q | q_stride) & 7u) || (((uintptr_t)d_out | out_stride | (uintptr_t)d_oq | oq_stride | (uintptr_t)d_len | (uintptr_t)d_seq) & 3u) || !aligned16(d_scratch))
     return fail(IE_B200_E_ARG, "ie_b200_attn_decode_paged: alignment (q 8 bytes, outputs 4, scratch 16)");
+  if (fill > 3u) return fail(IE_B200_E_ARG, "ie_b200_attn_decode_paged_fill: fill %u (0 to 3)", fill);
   const uint32_t hd = pages->hd, n_kv = pages->n_kv;
   if (n_head == 0 || n_head % n_kv || n_head > 65535u) return fail(IE_B200_E_SIZE, "ie_b200_attn_decode_paged: %u heads over %u KV heads", n_head, n_kv);
   if (hd != 32 && hd != 64 && hd != 128) return fail(IE_B200_E_SIZE, "ie_b200_attn_decode_paged: head dim %u unsupported (32, 64, 128)", hd);
@@ -808,7 +817,7 @@ extern "C" int ie_b200_attn_decode_paged(const float *d_q, const ie_b200_kv_page
   a.most = (uint32_t)(((1ull << 31) - 1u) / numbers);
   a.q = d_q, a.out = d_out, a.oq = static_cast<uint8_t *>(d_oq), a.len = d_len, a.seq = d_seq, a.err = d_err, a.kv = *pages;
   a.count = static_cast<uint32_t *>(d_scratch), a.rec = reinterpret_cast<float *>(static_cast<char *>(d_scratch) + AP_COUNT_BYTES);
-  a.n_head = n_head, a.G = n_head / n_kv, a.groups = groups, a.gw = (a.G + a.groups - 1u) / a.groups, a.R = R;
+  a.n_head = n_head, a.G = n_head / n_kv, a.groups = groups, a.gw = (a.G + a.groups - 1u) / a.groups, a.R = R, a.fill = fill;
   a.wide = (((uintptr_t)d_out | out_stride) & 15u) == 0u;
   a.q_stride = q_stride, a.out_stride = out_stride, a.oq_stride = oq_stride;
   a.scale_log2 = 1.44269504088896340736f / sqrtf((float)hd);

@@ -30,7 +30,7 @@ struct RopePagedArgs {
   const uint32_t *pos, *seq;
   uint32_t *err;
   ie_b200_kv_pages kv;
-  uint32_t nq, n_rope;
+  uint32_t nq, n_rope, fill;
   size_t stride, q_out_stride;
 };
 
@@ -71,19 +71,21 @@ __global__ void __launch_bounds__(256) rope_kv_paged_kernel(const RopePagedArgs 
   pdl_prologue();
   const uint32_t t = blockIdx.x, hd = a.kv.hd, h2 = hd / 2u, nkv = a.kv.n_kv;
   const uint32_t pos = a.pos[t], seq = a.seq ? a.seq[t] : t;
-  if (seq >= a.kv.n_seq) return;  // a row that pads the batch
-  const uint32_t col = pos / a.kv.page;
-  const uint32_t number = pos < table_positions(a.kv) && pos < a.n_rope ? page_number(a.kv, seq, col) : 0xFFFFFFFFu;
+  const bool real = seq < a.kv.n_seq;  // (else a row that pads the batch)
+  const uint32_t col = pos / a.kv.page, i = threadIdx.x * W, at0 = neox ? i : 2u * i, at1 = at0 + (neox ? h2 : W);  // i: first pair; at0, at1: first dimension of the two runs
+  float *qo = reinterpret_cast<float *>(reinterpret_cast<char *>(a.q_out) + a.q_out_stride * t);
+  const uint32_t number = real && pos < table_positions(a.kv) && pos < a.n_rope ? page_number(a.kv, seq, col) : 0xFFFFFFFFu;
   if (number >= a.kv.n_pages) {
-    if (a.err && threadIdx.x == 0 && threadIdx.y == 0) atomicExch(a.err, ERR_PAGES);
+    if (real && a.err && threadIdx.x == 0 && threadIdx.y == 0) atomicExch(a.err, ERR_PAGES);
+    const Floats<W> zero = {};
+    for (uint32_t h = blockIdx.y * blockDim.y + threadIdx.y; a.fill && h < a.nq; h += gridDim.y * blockDim.y)
+      st_row<W>(qo + (size_t)h * hd + at0, zero), st_row<W>(qo + (size_t)h * hd + at1, zero);
     return;
   }
-  const uint32_t i = threadIdx.x * W, at0 = neox ? i : 2u * i, at1 = at0 + (neox ? h2 : W);  // first pair; first dimension of the two runs
   const Floats<W> c = ld_floats<W>(a.cs + (size_t)pos * h2 + i), s = ld_floats<W>(a.sn + (size_t)pos * h2 + i);
   const size_t row0 = page_row(a.kv, number, 0u, pos - col * a.kv.page, hd * (uint32_t)sizeof(KV)), head_step = (size_t)a.kv.page * hd * sizeof(KV);
   const float *q = reinterpret_cast<const float *>(reinterpret_cast<const char *>(a.q) + a.stride * t), *k = reinterpret_cast<const float *>(reinterpret_cast<const char *>(a.k) + a.stride * t),
               *v = reinterpret_cast<const float *>(reinterpret_cast<const char *>(a.v) + a.stride * t);
-  float *qo = reinterpret_cast<float *>(reinterpret_cast<char *>(a.q_out) + a.q_out_stride * t);
   for (uint32_t h = blockIdx.y * blockDim.y + threadIdx.y; h < a.nq + 2u * nkv; h += gridDim.y * blockDim.y) {
     const bool is_q = h < a.nq, is_v = h >= a.nq + nkv;
     const uint32_t g = is_q ? h : is_v ? h - a.nq - nkv : h - a.nq;
@@ -133,15 +135,22 @@ using namespace ieb;
 extern "C" int ie_b200_rope_kv_paged(const float *d_q, const float *d_k, const float *d_v, float *d_q_out, const ie_b200_kv_pages *pages, const float *d_cos,
                                      const float *d_sin, uint32_t n_rope, const uint32_t *d_pos, const uint32_t *d_seq, uint32_t nq, int neox, uint32_t T,
                                      size_t qkv_stride, size_t q_out_stride, uint32_t *d_err, void *stream) {
+  return ie_b200_rope_kv_paged_fill(d_q, d_k, d_v, d_q_out, pages, d_cos, d_sin, n_rope, d_pos, d_seq, nq, neox, T, qkv_stride, q_out_stride, d_err, 0u, stream);
+}
+
+extern "C" int ie_b200_rope_kv_paged_fill(const float *d_q, const float *d_k, const float *d_v, float *d_q_out, const ie_b200_kv_pages *pages, const float *d_cos,
+                                          const float *d_sin, uint32_t n_rope, const uint32_t *d_pos, const uint32_t *d_seq, uint32_t nq, int neox, uint32_t T,
+                                          size_t qkv_stride, size_t q_out_stride, uint32_t *d_err, uint32_t fill, void *stream) {
   if (T == 0) return IE_B200_OK;  // (an empty tensor may have no address)
   if (int r = check_pages("ie_b200_rope_kv_paged", pages, 1u)) return r;
   if ((nq && (!d_q || !d_q_out)) || !d_k || !d_v || !d_cos || !d_sin || !d_pos) return fail(IE_B200_E_ARG, "ie_b200_rope_kv_paged: NULL pointer");
   if (((uintptr_t)d_q | (uintptr_t)d_k | (uintptr_t)d_v | (uintptr_t)d_q_out | (uintptr_t)d_cos | (uintptr_t)d_sin | (uintptr_t)d_pos | (uintptr_t)d_seq | qkv_stride | q_out_stride) & 3u)
     return fail(IE_B200_E_ARG, "ie_b200_rope_kv_paged: pointers and strides must be 4-byte aligned");
+  if (fill > 1u) return fail(IE_B200_E_ARG, "ie_b200_rope_kv_paged_fill: fill %u is neither 0 nor 1", fill);
   if (nq > 65535u) return fail(IE_B200_E_SIZE, "ie_b200_rope_kv_paged: %u query heads", nq);
   if (T > 0x7FFFFFFFu || (T > 1u && (qkv_stride < (size_t)pages->n_kv * pages->hd * 4u || (nq && q_out_stride < (size_t)nq * pages->hd * 4u))))
     return fail(IE_B200_E_SIZE, "ie_b200_rope_kv_paged: %u tokens with rows %zu and %zu bytes apart", T, qkv_stride, q_out_stride);
-  RopePagedArgs a = {d_q, d_k, d_v, d_cos, d_sin, d_q_out, d_pos, d_seq, d_err, *pages, nq, n_rope, qkv_stride, q_out_stride};
+  RopePagedArgs a = {d_q, d_k, d_v, d_cos, d_sin, d_q_out, d_pos, d_seq, d_err, *pages, nq, n_rope, fill, qkv_stride, q_out_stride};
   const bool wide = (((uintptr_t)d_q | (uintptr_t)d_k | (uintptr_t)d_v | (uintptr_t)d_q_out | (uintptr_t)d_cos | (uintptr_t)d_sin | qkv_stride | q_out_stride) & 15u) == 0u;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (pages->kv_f32) return wide ? launch_rope_paged<float, 4>(a, neox, T, st) : launch_rope_paged<float, 1>(a, neox, T, st);

@@ -371,7 +371,8 @@ def rope_kv_paged(qkv: torch.Tensor, kp: torch.Tensor, vp: torch.Tensor, table: 
                   seq: torch.Tensor | None, nq: int, nkv: int, hd: int, neox: bool, out: torch.Tensor | None = None, err: torch.Tensor | None = None) -> torch.Tensor:
     """New tokens of many sequences: qkv [T, (nq + 2 nkv) hd] f32 un-rotated (not changed); token t is position pos[t] of sequence
     seq[t] (None: of sequence t). Stores the rotated k and v into the pages and returns the rotated q [T, nq hd] (in `out` if given).
-    A seq[t] of n_seq or more (-1 too) marks a token that only pads the batch: nothing is done for it."""
+    A seq[t] of n_seq or more (-1 too) marks a token that only pads the batch: nothing is stored for it. Its row of q, and that of a token
+    whose position does not exist, is left as it was in a given `out`, zeros in a new one."""
     pages, dev, kv_heads, kv_hd, n_seq = _kv_pages(kp, vp, table)
     if nkv != kv_heads or hd != kv_hd:
         raise ValueError(f"{nkv} KV heads of {hd} against pools of {kv_heads} heads of {kv_hd}")
@@ -380,13 +381,14 @@ def rope_kv_paged(qkv: torch.Tensor, kp: torch.Tensor, vp: torch.Tensor, table: 
     if row != half:
         _refuse("cos", cos, _F32, (None, half), dev, "contiguous")
     s, p, q = _flat("sin", sin, _F32, (n_rope, half), dev), _flat("pos", pos, _I32, (T,), dev), _seq(seq, T, n_seq, dev)
-    if out is None:
+    fill = out is None
+    if fill:
         out, out_step = qkv.new_empty_strided((T, nq * hd), (nq * hd, 1)), nq * hd  # (two thirds of the time of torch.empty)
         to = out.data_ptr()
     else:
         to, _, _, out_step = _rows("out", out, _F32, T, nq * hd, dev)
-    _run(_lib.load().ie_b200_rope_kv_paged, dev, (base, base + 4 * nq * hd, base + 4 * (nq + nkv) * hd, to, pages, c, s, n_rope, p, q, nq, 1 if neox else 0, T, step * 4,
-                                                  out_step * 4, None if err is None else _flat("err", err, _I32, (1,), dev)))
+    _run(_lib.load().ie_b200_rope_kv_paged_fill, dev, (base, base + 4 * nq * hd, base + 4 * (nq + nkv) * hd, to, pages, c, s, n_rope, p, q, nq, 1 if neox else 0, T, step * 4,
+                                                       out_step * 4, None if err is None else _flat("err", err, _I32, (1,), dev), 1 if fill else 0))
     return out
 
 
@@ -402,20 +404,21 @@ def attn_decode_paged(q: torch.Tensor, kp: torch.Tensor, vp: torch.Tensor, table
                       seq: torch.Tensor | None = None, quant: bool = True, out: torch.Tensor | None = None, err: torch.Tensor | None = None):
     """One query token per row: q [R, n_head hd] f32 (rotated), row r sees the first lens[r] positions of sequence seq[r] (None: of
     sequence r). Returns (out [R, n_head hd], Q8 copies or None); a row that sees nothing is zeros, a row whose seq[r] is n_seq or
-    more (-1 too) is left as it was."""
+    more (-1 too) is left as it was in a given `out`, zeros in a new one and in the Q8 copies."""
     pages, dev, n_kv, hd, n_seq = _kv_pages(kp, vp, table)
     at, R, _, step = _rows("q", q, _F32, None, n_head * hd, dev)
     if scratch.layout != (n_head, n_kv, hd) or scratch.dev != dev:
         raise ValueError(f"scratch for {scratch.layout} (heads, KV heads, head size) on {scratch.data.device}, not {(n_head, n_kv, hd)} on cuda:{dev}")
     n, sq, row, nbq = _flat("lens", lens, _I32, (R,), dev), _seq(seq, R, n_seq, dev), n_head * hd, n_head * hd // 32
+    fill = 2 if out is not None else 3
     if out is None:
         out, out_step = torch.empty_like(q) if step == row else q.new_empty_strided((R, row), (row, 1)), row
         to = out.data_ptr()
     else:
         to, _, _, out_step = _rows("out", out, _F32, R, row, dev)
     oq = torch.empty((R, q8_bytes(nbq)), dtype=torch.uint8, device=q.device) if quant else None
-    _run(_lib.load().ie_b200_attn_decode_paged, dev, (at, pages, to, _p(oq), n, sq, n_head, R, step * 4, out_step * 4, q8_bytes(nbq), scratch.at,
-                                                      None if err is None else _flat("err", err, _I32, (1,), dev)))
+    _run(_lib.load().ie_b200_attn_decode_paged_fill, dev, (at, pages, to, _p(oq), n, sq, n_head, R, step * 4, out_step * 4, q8_bytes(nbq), scratch.at,
+                                                           None if err is None else _flat("err", err, _I32, (1,), dev), fill))
     return out, oq
 
 

@@ -168,7 +168,7 @@ int ie_b200_block_dots(int kind, const void *d_w, uint32_t rows, uint32_t cols, 
  * d_tok: T token ids on the device, each of them a row of the matrix (nothing checks that; 0xFFFFFFFF alone gives zeros). */
 int ie_b200_embed(int kind, const void *d_w, uint32_t cols, const uint32_t *d_tok, float *d_out, uint32_t T, size_t out_stride,
                   void *stream);
-/* The same for tokens that come from the device, from ie_b200_sample or ie_b200_argmax: a token of `rows` (of the matrix) or more, such
+/* The same for tokens that come from the device, from ie_b200_sample: a token of `rows` (of the matrix) or more, such
  * as the 0xFFFFFFFF of a row with nothing to draw or of one that pads a batch, gives a row of zeros. */
 int ie_b200_embed_rows(int kind, const void *d_w, uint32_t rows, uint32_t cols, const uint32_t *d_tok, float *d_out, uint32_t T,
                        size_t out_stride, void *stream);
@@ -280,6 +280,11 @@ typedef struct {
 int ie_b200_rope_kv_paged(const float *d_q, const float *d_k, const float *d_v, float *d_q_out, const ie_b200_kv_pages *pages, const float *d_cos,
                           const float *d_sin, uint32_t n_rope, const uint32_t *d_pos, const uint32_t *d_seq, uint32_t nq, int neox, uint32_t T,
                           size_t qkv_stride, size_t q_out_stride, uint32_t *d_err, void *stream);
+/* The same for a d_q_out that is new memory: with fill 1 the rows that would be left as they were (padding, positions that do not
+ * exist) are zeros. */
+int ie_b200_rope_kv_paged_fill(const float *d_q, const float *d_k, const float *d_v, float *d_q_out, const ie_b200_kv_pages *pages, const float *d_cos,
+                               const float *d_sin, uint32_t n_rope, const uint32_t *d_pos, const uint32_t *d_seq, uint32_t nq, int neox, uint32_t T,
+                               size_t qkv_stride, size_t q_out_stride, uint32_t *d_err, uint32_t fill, void *stream);
 
 /* Attention of R rows, one query token each, over the pages: row r sees positions 0 .. d_len[r] - 1 of sequence d_seq[r]
  * (d_seq NULL: of sequence r). Several rows may name one sequence (the tokens of a prompt, of a draft). A row that sees
@@ -295,6 +300,11 @@ size_t ie_b200_attn_decode_paged_scratch_bytes(uint32_t n_head, uint32_t n_kv, u
 int ie_b200_attn_decode_paged(const float *d_q, const ie_b200_kv_pages *pages, float *d_out, void *d_oq, const uint32_t *d_len, const uint32_t *d_seq,
                               uint32_t n_head, uint32_t R, size_t q_stride, size_t out_stride, size_t oq_stride, void *d_scratch, uint32_t *d_err,
                               void *stream);
+/* The same for outputs that are new memory: the rows that pad the batch are zeros in d_out (fill 1), in d_oq (2) or in both (3), and left
+ * as they were in the others. */
+int ie_b200_attn_decode_paged_fill(const float *d_q, const ie_b200_kv_pages *pages, float *d_out, void *d_oq, const uint32_t *d_len, const uint32_t *d_seq,
+                                   uint32_t n_head, uint32_t R, size_t q_stride, size_t out_stride, size_t oq_stride, void *d_scratch, uint32_t *d_err,
+                                   uint32_t fill, void *stream);
 
 /* First index of the maximum of each of T rows, and the softmax probability
  * of that maximum: OP_ARGMAX (src/cpu.c:608-614), ie_argmax
@@ -320,10 +330,10 @@ int ie_b200_topk(const float *d_x, uint32_t nv, uint32_t K, uint32_t T, size_t x
  * counts as 0, 1 and more as just below 1); the probability is w_i over that sum. temp 0 (or less, or NaN): the first maximum,
  * probability 1; a temp below 2^-126 counts as that. Weights are integers of 2^-44 of the largest one (2^-43 above 2^18 tokens; finer
  * for shorter rows), their sums exact; a token whose weight rounds to 0 is not drawn. A NaN logit is never drawn, one of -inf neither,
- * nor one that is further from the maximum than a float reaches; a row with nothing else gives index 0xFFFFFFFF and probability 0 (a token
- * that only ie_b200_embed_rows takes); where
- * the maximum is +inf its tokens are equally likely. d_u: T uniform numbers in [0, 1). d_temp, d_top_k, d_top_p, d_min_p: T values
- * each, or NULL (1, 0, 1, 0). n up to 360448, T up to 2^20. No scratch. The role of the reference's host sampler behind
+ * nor one that is further from the maximum than a float reaches; a row with nothing else gives index 0xFFFFFFFF and probability 0 (a
+ * token that ie_b200_embed_rows takes, ie_b200_embed does not); where the maximum is +inf its tokens are equally likely. d_u: T uniform
+ * numbers in [0, 1). d_temp, d_top_k, d_top_p, d_min_p: T values each, or NULL (1, 0, 1, 0). n up to 360448, T up to 2^20. No scratch.
+ * The role of the reference's host sampler behind
  * backend.topk (src/gen.c, src/backend.h:33-37), which knows temp and top_k. */
 int ie_b200_sample(const float *d_x, uint32_t n, uint32_t *d_idx, float *d_prob, const float *d_u, const float *d_temp, const uint32_t *d_top_k,
                    const float *d_top_p, const float *d_min_p, uint32_t T, size_t x_stride, void *stream);

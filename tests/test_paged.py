@@ -100,3 +100,10 @@ def test_sample_no_rows(lib):
     assert sample(lib, T=0) == 0 and lib.ie_b200_launch_count() == before
     with pytest.raises(ValueError, match="x"):
         K.sample(torch.zeros(1, 10), torch.zeros(1))
+
+
+def test_fill_is_refused_beyond_its_outputs(lib):
+    assert lib.ie_b200_rope_kv_paged_fill(AT, AT, AT, AT, pages(), AT, AT, 80, AT, None, 32, 0, 1, 48 * 512, 32 * 512, None, 2, None) == ARG
+    assert b"ie_b200_rope_kv_paged_fill" in lib.ie_b200_last_error()
+    assert lib.ie_b200_attn_decode_paged_fill(AT, pages(), AT, None, AT, None, 32, 1, 4096 * 4, 4096 * 4, 5120, AT, None, 4, None) == ARG
+    assert b"ie_b200_attn_decode_paged_fill" in lib.ie_b200_last_error()
