@@ -100,7 +100,9 @@ __device__ __forceinline__ void ap_split2(float x, float y, uint32_t &hi, uint32
   hi = *reinterpret_cast<const uint32_t *>(&h), lo = *reinterpret_cast<const uint32_t *>(&l);
 }
 
-// ---- a warp's part of the arithmetic: its running maximum (log2 units), sum and outputs of the unit's heads
+// ---- a warp's part of the arithmetic: its running maximum, sum and outputs of the unit's heads. The maximum is a score as it was summed, before the
+// factor to powers of two: the difference of the largest one to it is 0 and its weight 1, however large scores are (a maximum rounded after the factor
+// is off by half a unit in its last place, a whole power of two from 2^25 on, and a weight above 1 leaves half's range).
 template <typename KV, int HD, int W>
 struct ApWarp;
 
@@ -162,12 +164,12 @@ struct ApWarp<__half, HD, W> {
       mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 4));
       mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 8));
       mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 16));
-      const float m_new = fmaxf(m[j], mx * scale_log2), base = m_new == -INFINITY ? 0.0f : m_new;
-      al[j] = ex2(m[j] - base);
+      const float m_new = fmaxf(m[j], mx), base = m_new == -INFINITY ? 0.0f : m_new;
+      al[j] = ex2((m[j] - base) * scale_log2);
       float sum = 0.0f;
 #pragma unroll
       for (int n = 0; n < N; n++) {  // from here on the weights
-        s[n][j] = ex2(fmaf(s[n][j], scale_log2, -base)), s[n][2 + j] = ex2(fmaf(s[n][2 + j], scale_log2, -base));
+        s[n][j] = ex2((s[n][j] - base) * scale_log2), s[n][2 + j] = ex2((s[n][2 + j] - base) * scale_log2);
         sum += s[n][j] + s[n][2 + j];
       }
       l[j] = fmaf(l[j], al[j], sum);  // (of this lane's positions: the lanes meet in finish())
@@ -289,9 +291,9 @@ struct ApWarp<float, HD, W> {
       mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 4));
       mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 8));
       mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 16));
-      const float m_new = fmaxf(m[i], mx * scale_log2), base = m_new == -INFINITY ? 0.0f : m_new;
-      al_own[i] = ex2(m[i] - base);
-      w_own[i] = ex2(fmaf(x, scale_log2, -base));
+      const float m_new = fmaxf(m[i], mx), base = m_new == -INFINITY ? 0.0f : m_new;
+      al_own[i] = ex2((m[i] - base) * scale_log2);
+      w_own[i] = ex2((x - base) * scale_log2);
       l[i] = fmaf(l[i], al_own[i], w_own[i]);  // (of this lane's position: the lanes meet in finish())
       m[i] = m_new;
     }
@@ -640,7 +642,7 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int k = 0; k < WARPS; k++) {
-          const float f = ex2(ml[k * AP_HEADS * 2 + 2 * h] - base);
+          const float f = ex2((ml[k * AP_HEADS * 2 + 2 * h] - base) * a.scale_log2);
           const float4 v = *reinterpret_cast<const float4 *>(red + k * AP_HEADS * HD + Gm::red_at(h, d));
           L = fmaf(f, ml[k * AP_HEADS * 2 + 2 * h + 1], L);
           acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
@@ -693,7 +695,7 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
 #pragma unroll
                   for (uint32_t o = 1; o < QUADS; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
                   const float M_new = fmaxf(M, m), base = M_new == -INFINITY ? 0.0f : M_new;
-                  old = ex2(M - base), f = ex2(e.x - base);
+                  old = ex2((M - base) * a.scale_log2), f = ex2((e.x - base) * a.scale_log2);
                   float l = f * e.y;
 #pragma unroll
                   for (uint32_t o = 1; o < QUADS; o <<= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
