@@ -15,8 +15,9 @@
 //
 // Half cache: mma.sync m16n8k16, the positions on the 16-row side, the heads on the 8-column side (as attn_decode.cu). q and the
 // weights are carried as two f16 terms; every accumulation takes few MMAs (what the tensor cores cut off grows with their number) and is
-// added up in fp32: S in three chains (low terms, even and odd steps of the high ones), O per chunk. Weights are scaled by 2^15
-// before they are split, so that the low term of a small one keeps its bits (f16's subnormals end at 2^-24).
+// added up in fp32: S in three chains (low terms, even and odd steps of the high ones), O per chunk. f16's subnormals end at 2^-24, so both are
+// scaled before they are split, for the low terms to keep their bits: the weights by 2^15, a head's q by the power of two that takes its largest
+// value to 2^14 .. 2^15 (22 bits of every value down to 2^-17 of the largest, 2^-39 of that below, whatever q's size is).
 // Float cache: the same with fp32 FMAs, four lanes per position.
 //
 // Measured (half cache, heads of 128): 256 rows of 1000 positions, 32 x 8 heads, 164 us = 6.4 TB/s, 98 % of the measured copy rate; 64 rows of 1 to
@@ -100,9 +101,10 @@ __device__ __forceinline__ void ap_split2(float x, float y, uint32_t &hi, uint32
   hi = *reinterpret_cast<const uint32_t *>(&h), lo = *reinterpret_cast<const uint32_t *>(&l);
 }
 
-// ---- a warp's part of the arithmetic: its running maximum, sum and outputs of the unit's heads. The maximum is a score as it was summed, before the
-// factor to powers of two: the difference of the largest one to it is 0 and its weight 1, however large scores are (a maximum rounded after the factor
-// is off by half a unit in its last place, a whole power of two from 2^25 on, and a weight above 1 leaves half's range).
+// ---- a warp's part of the arithmetic: its running maximum (log2 units), sum and outputs of the unit's heads. log2(e) / sqrt(hd) is multiplied into q, so that a
+// score is in powers of two as it is summed (half cache: but for a whole power of two). The difference of the largest one to the maximum is then 0 and its weight
+// 1, however large scores are; a maximum rounded after such a factor is off by half a unit in its last place, a whole power of two from 2^25 on, and
+// a weight above 1 leaves half's range.
 template <typename KV, int HD, int W>
 struct ApWarp;
 
@@ -113,6 +115,7 @@ struct ApWarp<__half, HD, W> {
   float2 q[KS][2];                // the next unit's q, on its way
   uint32_t qh[KS][2], ql[KS][2];  // B fragments of Q^T[16 dims x heads]: column lane / 4
   float o[KS][4], m[2], l[2];     // o[u][j], o[u][2 + j]: head 2 (lane % 4) + j, dims 16 u + lane / 4, + 8
+  float unit[2];                  // what a sum for head 2 (lane % 4) + j counts for, a power of two
 
   __device__ __forceinline__ void load(const float *src, uint32_t heads, uint32_t tid) {
     const uint32_t h = (tid & 31u) >> 2, tq = tid & 3u;
@@ -121,11 +124,28 @@ struct ApWarp<__half, HD, W> {
 #pragma unroll
       for (int e = 0; e < 2; e++) q[k][e] = h < heads ? *reinterpret_cast<const float2 *>(src + h * HD + 16 * k + 2 * tq + 8 * e) : make_float2(0.f, 0.f);
   }
-  __device__ __forceinline__ void start(uint32_t, float *, uint32_t) {
+  __device__ __forceinline__ void start(float scale_log2, uint32_t lane) {
+    float part[2 * KS];  // (fmaxf passes over a NaN)
+#pragma unroll
+    for (int k = 0; k < KS; k++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) part[2 * k + e] = fmaxf(fabsf(q[k][e].x), fabsf(q[k][e].y));
+#pragma unroll
+    for (int n = KS; n; n >>= 1)
+#pragma unroll
+      for (int i = 0; i < n; i++) part[i] = fmaxf(part[i], part[i + n]);
+    float big = fmaxf(part[0], __shfl_xor_sync(0xFFFFFFFFu, part[0], 1));  // of head lane / 4
+    big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2)) * scale_log2;
+    // The power of two, times 2^127, that takes it to 2^14 .. 2^15; at most 2^100 (a q that small leaves all weights alike). A score takes it back, up to 2^88 of
+    // what can be 2^38: above that a head has all its weight on its largest scores either way, and nothing passes fp32's end.
+    const uint32_t up = min(268u - (__float_as_uint(big) >> 23), 227u), down = min(254u - up, 215u);
+    const float scale = scale_log2 * __uint_as_float(up << 23);
+#pragma unroll
+    for (uint32_t j = 0; j < 2; j++) unit[j] = __uint_as_float(__shfl_sync(0xFFFFFFFFu, down, 8u * (lane & 3u) + 4u * j) << 23);
 #pragma unroll
     for (int k = 0; k < KS; k++) {
 #pragma unroll
-      for (int e = 0; e < 2; e++) ap_split2(q[k][e].x, q[k][e].y, qh[k][e], ql[k][e]);
+      for (int e = 0; e < 2; e++) ap_split2(q[k][e].x * scale, q[k][e].y * scale, qh[k][e], ql[k][e]);
 #pragma unroll
       for (int e = 0; e < 4; e++) o[k][e] = 0.0f;
     }
@@ -133,7 +153,7 @@ struct ApWarp<__half, HD, W> {
   }
   // N chunks at once, each with `valid` positions
   template <int N>
-  __device__ __forceinline__ void chunks(const uint8_t *const (&stage)[N], const uint32_t (&valid)[N], float scale_log2, int lane) {
+  __device__ __forceinline__ void chunks(const uint8_t *const (&stage)[N], const uint32_t (&valid)[N], int lane) {
     const uint32_t lm = lane >> 3, lr = lane & 7, hq = lane >> 2;
     float s[N][4], al[2];  // s[.][j]: position lane / 4, s[.][2 + j]: + 8, of head 2 (lane % 4) + j
     float sl[N][4] = {}, s0[N][4] = {}, s1[N][4] = {};
@@ -164,12 +184,12 @@ struct ApWarp<__half, HD, W> {
       mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 4));
       mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 8));
       mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 16));
-      const float m_new = fmaxf(m[j], mx), base = m_new == -INFINITY ? 0.0f : m_new;
-      al[j] = ex2((m[j] - base) * scale_log2);
+      const float m_new = fmaxf(m[j], mx * unit[j]), base = m_new == -INFINITY ? 0.0f : m_new;
+      al[j] = ex2(m[j] - base);
       float sum = 0.0f;
 #pragma unroll
       for (int n = 0; n < N; n++) {  // from here on the weights
-        s[n][j] = ex2((s[n][j] - base) * scale_log2), s[n][2 + j] = ex2((s[n][2 + j] - base) * scale_log2);
+        s[n][j] = ex2(fmaf(s[n][j], unit[j], -base)), s[n][2 + j] = ex2(fmaf(s[n][2 + j], unit[j], -base));
         sum += s[n][j] + s[n][2 + j];
       }
       l[j] = fmaf(l[j], al[j], sum);  // (of this lane's positions: the lanes meet in finish())
@@ -197,10 +217,10 @@ struct ApWarp<__half, HD, W> {
       for (int e = 0; e < 4; e++) o[u][e] = fmaf(o[u][e], al[e & 1], c[e]);
     }
   }
-  __device__ __forceinline__ void chunk(const uint8_t *stage, uint32_t valid, float scale_log2, int lane) {
+  __device__ __forceinline__ void chunk(const uint8_t *stage, uint32_t valid, int lane) {
     const uint8_t *const st[1] = {stage};
     const uint32_t v[1] = {valid};
-    chunks<1>(st, v, scale_log2, lane);
+    chunks<1>(st, v, lane);
   }
   // this warp's record: red [heads][HD] outputs (2^15 times; red_at), ml [heads][2]
   __device__ __forceinline__ void finish(float *red, float *ml, int lane) {
@@ -234,18 +254,18 @@ struct ApWarp<float, HD, W> {
     for (int i = 0; i < QPT; i++) q[i] = tid + 32u * W * i < heads * HD ? src[tid + 32u * W * i] : 0.0f;
   }
   // (All threads call it, behind a barrier after which nobody reads what is at q_smem.)
-  __device__ __forceinline__ void start(uint32_t heads, float *q_smem, uint32_t tid) {
+  __device__ __forceinline__ void start(uint32_t heads, float *q_smem, float scale_log2, uint32_t tid) {
 #pragma unroll
-    for (int i = 0; i < QPT; i++) q_smem[tid + 32u * W * i] = q[i];
+    for (int i = 0; i < QPT; i++) q_smem[tid + 32u * W * i] = q[i] * scale_log2;
     __syncthreads();
     clear(heads, q_smem);
   }
   // The same for one warp, q from where it is.
-  __device__ __forceinline__ void start_alone(const float *src, uint32_t heads, float *q_smem, uint32_t lane) {
+  __device__ __forceinline__ void start_alone(const float *src, uint32_t heads, float *q_smem, float scale_log2, uint32_t lane) {
 #pragma unroll 8
     for (uint32_t i = 4u * lane; i < heads * HD; i += 128u) {
       const float2 a = *reinterpret_cast<const float2 *>(src + i), b = *reinterpret_cast<const float2 *>(src + i + 2);
-      *reinterpret_cast<float4 *>(q_smem + i) = make_float4(a.x, a.y, b.x, b.y);
+      *reinterpret_cast<float4 *>(q_smem + i) = make_float4(a.x * scale_log2, a.y * scale_log2, b.x * scale_log2, b.y * scale_log2);
     }
     for (uint32_t i = heads * HD + lane; i < AP_HEADS * HD; i += 32u) q_smem[i] = 0.0f;
     __syncwarp();
@@ -261,7 +281,7 @@ struct ApWarp<float, HD, W> {
   }
   // H: heads worked on, 4 or 8 (half the arithmetic where the unit has no more than four)
   template <int H>
-  __device__ __forceinline__ void chunk_of(uint8_t *stage, uint32_t valid, float scale_log2, int lane) {
+  __device__ __forceinline__ void chunk_of(uint8_t *stage, uint32_t valid, int lane) {
     const uint32_t pos = lane >> 2, part = lane & 3;  // lane: a quarter of the dims of one position
     float s[H];
 #pragma unroll
@@ -292,8 +312,8 @@ struct ApWarp<float, HD, W> {
       mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 8));
       mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 16));
       const float m_new = fmaxf(m[i], mx), base = m_new == -INFINITY ? 0.0f : m_new;
-      al_own[i] = ex2((m[i] - base) * scale_log2);
-      w_own[i] = ex2((x - base) * scale_log2);
+      al_own[i] = ex2(m[i] - base);
+      w_own[i] = ex2(x - base);
       l[i] = fmaf(l[i], al_own[i], w_own[i]);  // (of this lane's position: the lanes meet in finish())
       m[i] = m_new;
     }
@@ -337,9 +357,9 @@ struct ApWarp<float, HD, W> {
         for (int d = 0; d < DPL; d++) o[h][d] = fmaf(w[h], v[d], o[h][d]);
     }
   }
-  __device__ __forceinline__ void chunk(uint8_t *stage, uint32_t valid, float scale_log2, int lane) {
-    if (few) chunk_of<4>(stage, valid, scale_log2, lane);
-    else chunk_of<8>(stage, valid, scale_log2, lane);
+  __device__ __forceinline__ void chunk(uint8_t *stage, uint32_t valid, int lane) {
+    if (few) chunk_of<4>(stage, valid, lane);
+    else chunk_of<8>(stage, valid, lane);
   }
   __device__ __forceinline__ void finish(float *red, float *ml, int lane) {
 #pragma unroll
@@ -576,10 +596,10 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
       uint32_t h0;
       const uint32_t heads = heads_of(c, h0);
       if constexpr (Gm::F16) {
-        w.start(heads, nullptr, tid);
+        w.start(a.scale_log2, lane);
       } else {
-        if (alone) w.start_alone(q_of(c, h0), heads, red + warp * AP_HEADS * HD, lane);  // (where its record goes)
-        else w.start(heads, reinterpret_cast<float *>(smem_ap + Gm::Q_OFF), tid);
+        if (alone) w.start_alone(q_of(c, h0), heads, red + warp * AP_HEADS * HD, a.scale_log2, lane);  // (where its record goes)
+        else w.start(heads, reinterpret_cast<float *>(smem_ap + Gm::Q_OFF), a.scale_log2, tid);
       }
       uint32_t j = c.j0 + lane_of;
       if constexpr (Gm::PAIRS) {
@@ -590,7 +610,7 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
           const uint8_t *const st[2] = {ring + stage * Gm::STAGE, ring + second * Gm::STAGE};
           const uint32_t valid[2] = {valid_of[stage], valid_of[second]};
           fetch();
-          w.template chunks<2>(st, valid, a.scale_log2, lane);
+          w.template chunks<2>(st, valid, lane);
           __syncwarp();
           fetch();
           stage = second + 1u == STAGES ? 0u : second + 1u;
@@ -601,7 +621,7 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
         __syncwarp();
         const uint32_t valid = valid_of[stage];
         fetch();
-        w.chunk(ring + stage * Gm::STAGE, valid, a.scale_log2, lane);
+        w.chunk(ring + stage * Gm::STAGE, valid, lane);
         stage = stage + 1u == STAGES ? 0u : stage + 1u;
       }
       // ---- the warps' records meet; the next unit's q sets out meanwhile
@@ -642,7 +662,7 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int k = 0; k < WARPS; k++) {
-          const float f = ex2((ml[k * AP_HEADS * 2 + 2 * h] - base) * a.scale_log2);
+          const float f = ex2(ml[k * AP_HEADS * 2 + 2 * h] - base);
           const float4 v = *reinterpret_cast<const float4 *>(red + k * AP_HEADS * HD + Gm::red_at(h, d));
           L = fmaf(f, ml[k * AP_HEADS * 2 + 2 * h + 1], L);
           acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
@@ -695,7 +715,7 @@ __global__ void __launch_bounds__(32 * W, ApGeom<KV, HD, W>::CTAS) attn_paged_ke
 #pragma unroll
                   for (uint32_t o = 1; o < QUADS; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
                   const float M_new = fmaxf(M, m), base = M_new == -INFINITY ? 0.0f : M_new;
-                  old = ex2((M - base) * a.scale_log2), f = ex2((e.x - base) * a.scale_log2);
+                  old = ex2(M - base), f = ex2(e.x - base);
                   float l = f * e.y;
 #pragma unroll
                   for (uint32_t o = 1; o < QUADS; o <<= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, o);

@@ -290,8 +290,8 @@ int ie_b200_rope_kv_paged_fill(const float *d_q, const float *d_k, const float *
  * (d_seq NULL: of sequence r). Several rows may name one sequence (the tokens of a prompt, of a draft). A row that sees
  * nothing (length 0) is zeros. The work is dealt out evenly over the GPU whatever the lengths are; where it cuts a (row, KV
  * head) into parts the last part to finish merges them, in a fixed order. What lies in rows of the pages that a row does not
- * see has no part in its result; an infinity or NaN in one that it sees may make NaN of its head, and so may a q beyond half's
- * range (65504) with half pools. Optional Q8 copies of the
+ * see has no part in its result; an infinity or NaN in one that it sees, or in q, may make NaN of its head (scores that are all -inf
+ * give zeros). q may be of any size whose scores a float holds, with half pools too. Optional Q8 copies of the
  * rows (d_oq). hd 32, 64 or 128, n_head a multiple of n_kv, pages of a multiple of 16 positions, at most 2^31 - 1 in a table row;
  * q 8-byte aligned, strides in bytes. d_scratch: ie_b200_attn_decode_paged_scratch_bytes() bytes of the device the call is
  * made on, 16-byte aligned, zero before the first call and left ready by every call; calls that share it (graphs that
