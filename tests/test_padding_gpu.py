@@ -1,5 +1,5 @@
-"""What a batched step makes of rows that only pad the batch and of rows with nothing to draw: no memory that is not the step's own is
-read or handed out."""
+"""What a batched step makes of rows that only pad the batch, of rows with nothing to draw and of memory that others have used: nothing that is
+not the step's own is read or handed out."""
 import numpy as np
 import pytest
 import torch
@@ -130,3 +130,21 @@ def test_padded_steps_fed_by_their_own_draws(cuda):
         graph.replay()
         look(*results)
         tok.copy_(results[3])
+
+
+def test_a_new_scratch_on_another_stream(cuda):
+    """A scratch made behind work that is still running is ready when a call on another stream uses it at once: the parts of a cut row are joined."""
+    gen = torch.Generator(device=cuda).manual_seed(2)
+    kp, vp = (torch.randn(40, 2, 16, 64, device=cuda, generator=gen).half() for _ in "kv")
+    table, lens = torch.randperm(40, device=cuda, generator=gen).int().view(1, 40), torch.tensor([640], dtype=torch.int32, device=cuda)
+    q = torch.randn(1, 8 * 64, device=cuda, generator=gen)
+    want, _ = K.attn_decode_paged(q, kp, vp, table, lens, 8, K.PagedScratch(8, 2, 64, cuda), quant=False)
+    size, side, out = K.PagedScratch(8, 2, 64, cuda).data.numel(), torch.cuda.Stream(), torch.zeros_like(q)
+    poison(((size,), torch.uint8))
+    torch.cuda._sleep(400_000_000)  # some 0.2 s on this stream
+    scratch = K.PagedScratch(8, 2, 64, cuda)
+    with torch.cuda.stream(side):
+        K.attn_decode_paged(q, kp, vp, table, lens, 8, scratch, quant=False, out=out)
+    side.synchronize()
+    assert torch.equal(out, want)
+    torch.cuda.synchronize()
