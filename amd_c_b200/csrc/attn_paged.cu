@@ -20,7 +20,7 @@
 // value to 2^14 .. 2^15 (22 bits of every value down to 2^-17 of the largest, 2^-39 of that below, whatever q's size is).
 // Float cache: the same with fp32 FMAs, four lanes per position.
 //
-// Measured (half cache, heads of 128): 256 rows of 1000 positions, 32 x 8 heads, 164 us = 6.4 TB/s, 98 % of the measured copy rate; 64 rows of 1 to
+// Measured (half cache, heads of 128): 256 rows of 1000 positions, 32 x 8 heads, 164 .. 167 us = 6.3 TB/s, 97 % of the measured copy rate; 64 rows of 1 to
 // 8192, 28 x 4, 91 us = 6.0 TB/s; 1 of 32768, 40 x 8, 29.3 us (the contiguous kernel of attn_decode.cu 34 us with 32 x 8), of which
 // 4 us are the start (length, page number, first rows: dependent round trips) and 4 the merge of 18 parts; 1 of 500, 8.1 us. Float cache, heads of
 // 128: 64 rows of up to 3001, 132 us = 6.3 TB/s; of 64: 253 rows of 868 141 us = 6.4 TB/s.
@@ -794,7 +794,8 @@ static int launch_ap(PagedAttnArgs &a, cudaStream_t st) {
 // 32768 positions of 8 KV heads 28.8 against 30.4 us, 1 x 4000 11.6 / 12.4; at 64 units, 8 x 8192 at most, 33.7 / 32.3), and with the half
 // cache where units have many heads and may be long (28 x 4 heads: 64 x 8192 at most 90.1 / 91.6, 32 x 4096 29.7 / 31.8; with 32 x 8
 // 172 / 168, 128 x 2500 at most 108 / 101). Four else: a unit's end waits for fewer warps (256 x 200 57 / 45; float cache, 64 x 3001 at most, 137 / 132).
-// What the host knows of the lengths is how wide the table is.
+// What the host knows of the lengths is how wide the table is; short rows of a wide one (8192 positions) get eight all the same: 256 x 200 of 28 x 4 heads 37
+// against 31 us, of 40 x 8 61 / 49, but 16 x 500 10.6 / 11.3 and 12.0 / 15.6.
 template <typename KV, int HD>
 static int launch_ap(PagedAttnArgs &a, cudaStream_t st) {
   const bool few = 4u * (uint64_t)a.R * a.kv.n_kv * a.groups <= (uint32_t)sm_count(), maybe_long = sizeof(KV) == 2 && a.gw > 4u && table_positions(a.kv) >= 2048u;
