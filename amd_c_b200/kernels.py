@@ -394,13 +394,13 @@ def rope_kv_paged(qkv: torch.Tensor, kp: torch.Tensor, vp: torch.Tensor, table: 
 
 class PagedScratch:
     """Counters and partial records of attn_decode_paged for one head layout, on one device, ready for any stream. One call at a time may
-    use it."""
+    use it. Made inside a capture it is that graph's (whose replays zero it first)."""
 
     def __init__(self, n_head: int, n_kv: int, hd: int, device):
         self.data = torch.zeros(_lib.load().ie_b200_attn_decode_paged_scratch_bytes(n_head, n_kv, hd), dtype=torch.uint8, device=device)
         self.layout, self.at, self.dev = (n_head, n_kv, hd), self.data.data_ptr(), self.data.get_device()
-        if not torch.cuda.is_current_stream_capturing():  # (in a graph the zeros are a part of it)
-            torch.cuda.current_stream(self.dev).synchronize()  # (the counters are zero before a call on another stream reads them)
+        if not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream(self.dev).synchronize()  # the counters are zero before a call on another stream reads them
 
 
 def attn_decode_paged(q: torch.Tensor, kp: torch.Tensor, vp: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, n_head: int, scratch: PagedScratch,

@@ -148,3 +148,18 @@ def test_a_new_scratch_on_another_stream(cuda):
     side.synchronize()
     assert torch.equal(out, want)
     torch.cuda.synchronize()
+
+
+def test_a_scratch_made_in_a_graph(cuda):
+    """A graph that makes its own scratch: every replay joins the parts of a cut row."""
+    gen = torch.Generator(device=cuda).manual_seed(3)
+    kp, vp = (torch.randn(40, 2, 16, 64, device=cuda, generator=gen).half() for _ in "kv")
+    table, lens = torch.randperm(40, device=cuda, generator=gen).int().view(1, 40), torch.tensor([640], dtype=torch.int32, device=cuda)
+    q, out = torch.randn(1, 8 * 64, device=cuda, generator=gen), torch.zeros(1, 8 * 64, device=cuda)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        K.attn_decode_paged(q, kp, vp, table, lens, 8, K.PagedScratch(8, 2, 64, cuda), quant=False, out=out)
+    for _ in range(3):
+        q.normal_(generator=gen), out.zero_()
+        graph.replay()
+        assert torch.equal(out, K.attn_decode_paged(q, kp, vp, table, lens, 8, K.PagedScratch(8, 2, 64, cuda), quant=False)[0])
